@@ -37,11 +37,11 @@ def listed():
         # a serving batch: 256 sequences, up to 64 drafts each, ragged
         dict(name="mask batch", op="mask", seqs=256, tokens=64, ctx=4000),
         # one sequence's 16 drafts of a 48/8-head layer: the smallest store
-        dict(name="store one", op="store", tokens=16, hq=48, hkv=8, rot=128, neox=True, v="q8t", dtype="bf16", ctx=8000),
-        # 64 sequences x 33 drafts, GPT-J pairs over half the head, 16-bit V, odd token count
-        dict(name="store batch", op="store", tokens=2111, hq=48, hkv=8, rot=64, neox=False, v="v16", dtype="fp16", ctx=32768),
+        dict(name="store one", op="store", tokens=16, run=16, hq=48, hkv=8, rot=128, neox=True, v="q8t", dtype="bf16", ctx=8000),
+        # 64 sequences of up to 33 drafts, GPT-J pairs over half the head, 16-bit V, odd token count
+        dict(name="store batch", op="store", tokens=2111, run=33, hq=48, hkv=8, rot=64, neox=False, v="v16", dtype="fp16", ctx=32768),
         # a prompt chunk that fills the cache before drafting starts
-        dict(name="store prompt", op="store", tokens=16384, hq=48, hkv=8, rot=128, neox=True, v="q8t", dtype="bf16", ctx=32768),
+        dict(name="store prompt", op="store", tokens=16384, run=16384, hq=48, hkv=8, rot=128, neox=True, v="q8t", dtype="bf16", ctx=32768),
         # one sequence, short context, small tree: latency of one layer
         dict(name="attention one", op="attention", seqs=1, lo=2047, hi=2047, tokens=8, hq=48, hkv=8, v="q8t", dtype="bf16",
              softcap=0.0, window=0),
@@ -72,7 +72,8 @@ def draw(rng):
     if op == "mask":
         return dict(op=op, seqs=_log(rng, 1, 256), tokens=_log(rng, 2, 64), ctx=_log(rng, 64, 32768))
     if op == "store":
-        return dict(op=op, tokens=_log(rng, 1, 16384), hq=hkv * rng.randint(1, 6), hkv=hkv, rot=rng.choice([32, 64, 96, 128]),
+        tokens = _log(rng, 1, 16384)
+        return dict(op=op, tokens=tokens, run=_log(rng, 1, tokens) if tokens > 1 else 1, hq=hkv * rng.randint(1, 6), hkv=hkv, rot=rng.choice([32, 64, 96, 128]),
                     neox=rng.random() < 0.6, v=rng.choice(["q8t", "v16"]), dtype=rng.choice(["bf16", "fp16"]),
                     ctx=_log(rng, 512, 32768))
     if op == "attention":
@@ -226,12 +227,20 @@ def prepare(case, seed):
         weights = 1 + 0.2 * torch.randn((2, D), device=DEV, generator=g)
         inv = 1.0 / (1e6 ** (torch.arange(0, case["rot"], 2, device=DEV, dtype=torch.float32) / case["rot"]))
         angle = torch.outer(torch.arange(case["ctx"], device=DEV, dtype=torch.float32), inv)
-        nb = -(-t // 16) + 4
+        # runs of `run` tokens, one a sequence: each starts somewhere inside a page of its own and goes on through its next pages
+        run, runs = case["run"], -(-t // case["run"])
+        per = -(-(run + 15) // 16)
+        first = torch.randint(0, 16, (runs,), device=DEV, generator=g)
+        base = torch.randint(0, max(1, case["ctx"] - run), (runs,), device=DEV, generator=g)
+        of, at = torch.arange(t, device=DEV) // run, torch.arange(t, device=DEV) % run
+        nb = runs * per + 1
+        pages = torch.randperm(nb - 1, device=DEV, generator=g) + 1
+        at_slot = first[of] + at
         kv = torch.zeros((nb, 2, 16, hkv, D), dtype=dt, device=DEV)
         k, v = _views(kv, case["v"])
-        slots = torch.randperm((nb - 1) * 16, device=DEV, generator=g)[:t] + 16
+        slots = pages[of * per + at_slot // 16] * 16 + at_slot % 16
         s |= {"q": qkv[:, :hq], "k": qkv[:, hq:hq + hkv], "v": qkv[:, hq + hkv:], "wq": weights[0].to(dt), "wk": weights[1].to(dt),
-              "pos": torch.randint(0, case["ctx"], (t,), device=DEV, generator=g), "cs": torch.cat([angle.cos(), angle.sin()], -1).to(dt),
+              "pos": (base[of] + at) % case["ctx"], "cs": torch.cat([angle.cos(), angle.sin()], -1).to(dt),
               "slots": slots, "kc": k, "vc": v, "q_out": torch.empty((t, hq, D), dtype=dt, device=DEV)}
         return s
     if op == "attention":
