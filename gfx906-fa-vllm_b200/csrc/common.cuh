@@ -24,7 +24,8 @@ __host__ __device__ inline int q8_row_bytes(int D) { return (D / QK) * QBLOCK; }
 // Error word written by device code when a bounded wait gives up or an
 // argument fails an in-kernel check.  Read/reset through the C ABI
 // (gfx906_fa_get_device_error).  Bit 0: mbarrier wait timed out; bit 1:
-// block-table entry out of range; bit 2: tensor-memory allocation failed.
+// block-table entry out of range; bit 2: tensor-memory allocation failed;
+// bit 3: a slot, position or parent link out of range.
 // Each translation unit has its own copy (no relocatable device code); the
 // C ABI ORs them together (see G9_ERROR_ACCESSORS).
 static __device__ unsigned int g_device_error;
@@ -33,6 +34,7 @@ enum DeviceError : unsigned int {
   ERR_WAIT_TIMEOUT = 1u,
   ERR_BAD_PAGE = 2u,
   ERR_TMEM = 4u,
+  ERR_BAD_INDEX = 8u,
 };
 
 __device__ __forceinline__ void raise_error(unsigned int bits) { atomicOr(&g_device_error, bits); }

@@ -1,0 +1,504 @@
+// norm_store.cu -- per-head RMS norm + rotation of queries and keys with the
+// Q8_0 store of keys and values in the same pass, and the reader of stored
+// rows (head size 128).
+//
+//   y = x * rsqrt(mean(x^2) + eps) * w          over the 128 elements of a head
+//   rotated pairs (a, b) of the first rot_dim elements:
+//     a' = a cos - b sin,  b' = b cos + a sin   (angles by the token's position)
+//   one rounding to the tensor's type; a key is quantised from that rounding
+//
+// Half a warp holds a row, 8 elements a lane, so every row is one 16-byte
+// load per lane, the mean of squares four shuffles and a Q8_0 block's maximum
+// two.  All arithmetic is fp32.  Bound by HBM: queries and keys are read and
+// written once, where separate norm, rotation and store passes move them
+// three times.
+#include "common.cuh"
+#include "gfx906_fa_b200.h"
+
+namespace g9 {
+
+struct NormStoreArgs {
+  const void* q; const void* k; const void* v;
+  void* q_out; void* k_out;                        // k_out may be null
+  int q_dt, k_dt, v_dt;
+  int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head;      // elements
+  int64_t qo_tok, qo_head, ko_tok, ko_head;
+  int q_vec, k_vec, v_vec, qo_vec, ko_vec;         // 1: rows start on 16-byte boundaries
+  const void* q_w; const void* k_w;                // null: no norm
+  int qw_dt, kw_dt;
+  float eps;
+  const int64_t* positions;
+  const void* cos_sin;                             // [max_pos, rot]: cos of pair j at j, sin at rot/2 + j
+  int cs_dt, rot, neox, cs_vec;
+  int64_t max_pos;
+  const int64_t* slots;
+  G9KvCache c;
+  int k_w8, v_w8, v_w16;                           // cache rows: 8-byte (K, Q8_0 V) / 16-byte (16-bit V) aligned
+  int T, Hq, Hkv, rows;                            // rows of a token: Hq + Hkv + (V stored ? Hkv : 0)
+  int rpw;                                         // rows of a token a half-warp takes
+};
+
+namespace ns {
+constexpr int D = 128;
+constexpr int WARPS = 8;
+constexpr int BATCH = 4;                           // rows in flight per half-warp
+constexpr int RB = D / QK * QBLOCK;
+}  // namespace ns
+
+// 8 consecutive elements of a row as loaded; fp32 rows take two registers quads
+struct Raw8 { uint4 a, b; };
+
+__device__ __forceinline__ Raw8 load_raw8(const void* p, int64_t i, int dt, bool vec) {
+  Raw8 r;
+  r.b = make_uint4(0, 0, 0, 0);
+  if (dt == DT_F32) {
+    const float* f = reinterpret_cast<const float*>(p) + i;
+    if (vec) {
+      r.a = reinterpret_cast<const uint4*>(f)[0];
+      r.b = reinterpret_cast<const uint4*>(f)[1];
+    } else {
+      const uint32_t* u = reinterpret_cast<const uint32_t*>(f);
+      r.a = make_uint4(u[0], u[1], u[2], u[3]);
+      r.b = make_uint4(u[4], u[5], u[6], u[7]);
+    }
+  } else {
+    const uint16_t* h = reinterpret_cast<const uint16_t*>(p) + i;
+    if (vec) r.a = *reinterpret_cast<const uint4*>(h);
+    else
+      r.a = make_uint4(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16, h[4] | (uint32_t)h[5] << 16,
+                       h[6] | (uint32_t)h[7] << 16);
+  }
+  return r;
+}
+
+__device__ __forceinline__ void widen8(const Raw8& r, int dt, float v[8]) {
+  const uint32_t w[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
+  if (dt == DT_F32) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(w[e]);
+  } else if (dt == DT_BF16) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      v[2 * e] = __uint_as_float(w[e] << 16);
+      v[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+      v[2 * e] = x.x;
+      v[2 * e + 1] = x.y;
+    }
+  }
+}
+
+// rounds v to dt (in place, back as fp32) and returns the packed 16-bit words (16-bit dt)
+__device__ __forceinline__ uint4 round8(float v[8], int dt) {
+  uint32_t w[4] = {0, 0, 0, 0};
+  if (dt == DT_F16) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const __half2 h = __floats2half2_rn(v[2 * e], v[2 * e + 1]);
+      w[e] = *reinterpret_cast<const uint32_t*>(&h);
+      const float2 x = __half22float2(h);
+      v[2 * e] = x.x;
+      v[2 * e + 1] = x.y;
+    }
+  } else if (dt == DT_BF16) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
+      w[e] = *reinterpret_cast<const uint32_t*>(&h);
+      v[2 * e] = __uint_as_float(w[e] << 16);
+      v[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// v already rounded to dt, `packed` its 16-bit words
+__device__ __forceinline__ void store8(void* p, int64_t i, int dt, bool vec, const float v[8], uint4 packed) {
+  if (dt == DT_F32) {
+    float* f = reinterpret_cast<float*>(p) + i;
+    if (vec) {
+      reinterpret_cast<float4*>(f)[0] = make_float4(v[0], v[1], v[2], v[3]);
+      reinterpret_cast<float4*>(f)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = v[e];
+    }
+  } else {
+    uint16_t* h = reinterpret_cast<uint16_t*>(p) + i;
+    if (vec) {
+      *reinterpret_cast<uint4*>(h) = packed;
+    } else {
+      const uint32_t w[4] = {packed.x, packed.y, packed.z, packed.w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) h[e] = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+    }
+  }
+}
+
+// Q8_0 of the 8 elements of this lane (a block is 4 neighbouring lanes): the
+// quantiser's arithmetic, element for element (IEEE division and reciprocal,
+// round half to even, clamp).
+__device__ __forceinline__ uint2 quant8(const float v[8], uint16_t& scale) {
+  float amax = fabsf(v[0]);
+#pragma unroll
+  for (int e = 1; e < 8; ++e) amax = fmaxf(amax, fabsf(v[e]));
+  amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+  amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+  const float d = amax / 127.0f;
+  const float id = d > 0.0f ? __frcp_rn(d) : 0.0f;
+  uint32_t w[2] = {0, 0};
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    int qi = __float2int_rn(v[e] * id);
+    qi = max(-128, min(127, qi));
+    w[e >> 2] |= (uint32_t)(qi & 0xff) << (8 * (e & 3));
+  }
+  scale = __half_as_ushort(__float2half_rn(d));
+  return make_uint2(w[0], w[1]);
+}
+
+// cos / sin of this lane's 8 elements.  NeoX: element e pairs with e +- rot/2;
+// otherwise 2j with 2j + 1, four pairs a lane.
+struct Angles { float c[8], s[8]; };
+
+__device__ __forceinline__ void load_angles(const NormStoreArgs& a, int64_t pos, int hl, Angles& g) {
+  const int half = a.rot >> 1, e0 = 8 * hl;
+  if (e0 >= a.rot) return;
+  const int64_t base = pos * a.rot;
+  const int j0 = a.neox ? (e0 < half ? e0 : e0 - half) : e0 >> 1;
+  if (a.neox) {
+    widen8(load_raw8(a.cos_sin, base + j0, a.cs_dt, a.cs_vec), a.cs_dt, g.c);
+    widen8(load_raw8(a.cos_sin, base + half + j0, a.cs_dt, a.cs_vec), a.cs_dt, g.s);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      g.c[e] = load_one(a.cos_sin, base + j0 + e, a.cs_dt);
+      g.s[e] = load_one(a.cos_sin, base + half + j0 + e, a.cs_dt);
+    }
+  }
+}
+
+__device__ __forceinline__ void rotate8(const NormStoreArgs& a, const Angles& g, int hl, float v[8]) {
+  const int e0 = 8 * hl;
+  if (a.neox) {
+    const int lanes = a.rot >> 4;                  // lanes per half of the rotated part
+    const bool lower = hl < lanes;
+    // the partner's lane; lanes past the rotated part read themselves
+    const int peer = e0 >= a.rot ? hl : lower ? hl + lanes : hl - lanes;
+    const int src = (threadIdx.x & 16) | peer;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float p = __shfl_sync(0xffffffffu, v[e], src);
+      if (e0 < a.rot)
+        v[e] = lower ? __fsub_rn(__fmul_rn(v[e], g.c[e]), __fmul_rn(p, g.s[e]))
+                     : __fadd_rn(__fmul_rn(v[e], g.c[e]), __fmul_rn(p, g.s[e]));
+    }
+  } else if (e0 < a.rot) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float x = v[2 * e], y = v[2 * e + 1];
+      v[2 * e] = __fsub_rn(__fmul_rn(x, g.c[e]), __fmul_rn(y, g.s[e]));
+      v[2 * e + 1] = __fadd_rn(__fmul_rn(y, g.c[e]), __fmul_rn(x, g.s[e]));
+    }
+  }
+}
+
+__device__ __forceinline__ void norm8(float v[8], const float w[8], float eps) {
+  float ss = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) ss += v[e] * v[e];
+#pragma unroll
+  for (int x = 1; x < 16; x <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, x);
+  const float r = rsqrtf(ss * (1.0f / ns::D) + eps);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = v[e] * r * w[e];
+}
+
+// Q8_0 row from the lanes' blocks: staged so that it leaves as 8-byte words
+__device__ __forceinline__ void write_q8_row(uint8_t* dst, uint2 w, uint16_t scale, int hl, bool live, bool w8,
+                                             uint8_t* stage) {
+  uint16_t* o = reinterpret_cast<uint16_t*>(stage + (hl >> 2) * QBLOCK + 2 + 8 * (hl & 3));
+  o[0] = (uint16_t)w.x; o[1] = (uint16_t)(w.x >> 16);
+  o[2] = (uint16_t)w.y; o[3] = (uint16_t)(w.y >> 16);
+  if ((hl & 3) == 0) *reinterpret_cast<uint16_t*>(stage + (hl >> 2) * QBLOCK) = scale;
+  __syncwarp();
+  if (live) {
+    if (w8) {
+      reinterpret_cast<uint64_t*>(dst)[hl] = reinterpret_cast<const uint64_t*>(stage)[hl];
+      if (hl == 0) reinterpret_cast<uint64_t*>(dst)[16] = reinterpret_cast<const uint64_t*>(stage)[16];
+    } else {
+      for (int i = hl; i < ns::RB / 2; i += 16)
+        reinterpret_cast<uint16_t*>(dst)[i] = reinterpret_cast<const uint16_t*>(stage)[i];
+    }
+  }
+  __syncwarp();
+}
+
+__global__ void __launch_bounds__(ns::WARPS * 32) norm_store_kernel(const __grid_constant__ NormStoreArgs a) {
+  using namespace ns;
+  __shared__ __align__(16) uint8_t stage_all[WARPS * 2][RB];
+  const int lane = lane_id(), hl = lane & 15;
+  uint8_t* stage = stage_all[warp_id() * 2 + (lane >> 4)];
+  const int chunks = (a.rows + a.rpw - 1) / a.rpw;
+  const int64_t items = (int64_t)a.T * chunks;
+  // both halves of a warp make the same trips: the shuffles and barriers below are warp-wide
+  for (int64_t i0 = ((int64_t)blockIdx.x * WARPS + warp_id()) * 2; i0 < items;
+       i0 += (int64_t)gridDim.x * WARPS * 2) {
+    const int64_t it = i0 + (lane >> 4);
+    const bool on = it < items;
+    const int t = on ? (int)(it / chunks) : 0;
+    const int r0 = on ? (int)(it % chunks) * a.rpw : 0;
+    const int nr = on ? min(a.rpw, a.rows - r0) : 0;
+    int64_t pos = a.positions[t];
+    const int64_t slot = a.slots[t];
+    if (pos < 0 || pos >= a.max_pos) {
+      raise_error(ERR_BAD_INDEX);
+      pos = 0;
+    }
+    int64_t blk = slot / a.c.block_size;
+    const int off = (int)(slot - blk * a.c.block_size);
+    bool stored = on && slot >= 0;
+    if (stored && a.c.num_blocks > 0 && blk >= a.c.num_blocks) {
+      raise_error(ERR_BAD_INDEX);
+      stored = false;
+    }
+    Angles g;
+    load_angles(a, pos, hl, g);
+    for (int b = 0; b < a.rpw; b += BATCH) {
+      Raw8 raw[BATCH];
+#pragma unroll
+      for (int x = 0; x < BATCH; ++x) {
+        const int r = r0 + b + x;
+        if (b + x >= a.rpw) break;
+        raw[x].a = raw[x].b = make_uint4(0, 0, 0, 0);
+        if (b + x < nr) {
+          if (r < a.Hq) raw[x] = load_raw8(a.q, (int64_t)t * a.q_tok + (int64_t)r * a.q_head + 8 * hl, a.q_dt, a.q_vec);
+          else if (r < a.Hq + a.Hkv)
+            raw[x] = load_raw8(a.k, (int64_t)t * a.k_tok + (int64_t)(r - a.Hq) * a.k_head + 8 * hl, a.k_dt, a.k_vec);
+          else
+            raw[x] = load_raw8(a.v, (int64_t)t * a.v_tok + (int64_t)(r - a.Hq - a.Hkv) * a.v_head + 8 * hl, a.v_dt, a.v_vec);
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < BATCH; ++x) {
+        const int r = r0 + b + x;
+        if (b + x >= a.rpw) break;                 // the same for the whole grid
+        const bool live = b + x < nr;
+        const bool isq = r < a.Hq, isv = r >= a.Hq + a.Hkv;
+        const int dt = isq ? a.q_dt : isv ? a.v_dt : a.k_dt;
+        float v[8];
+        widen8(raw[x], dt, v);
+        // every lane takes the shuffles; their results are used by live query and key rows only
+        const void* wp = isq ? a.q_w : a.k_w;
+        float w[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (wp) widen8(load_raw8(wp, 8 * hl, isq ? a.qw_dt : a.kw_dt, false), isq ? a.qw_dt : a.kw_dt, w);
+        float y[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = v[e];
+        norm8(y, w, a.eps);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = wp ? y[e] : v[e];
+        rotate8(a, g, hl, y);
+        if (!isv) {
+          const uint4 packed = round8(y, dt);
+          if (live) {
+            if (isq)
+              store8(a.q_out, (int64_t)t * a.qo_tok + (int64_t)r * a.qo_head + 8 * hl, dt, a.qo_vec, y, packed);
+            else if (a.k_out)
+              store8(a.k_out, (int64_t)t * a.ko_tok + (int64_t)(r - a.Hq) * a.ko_head + 8 * hl, dt, a.ko_vec, y, packed);
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = y[e];
+        }
+        // ---- cache rows -------------------------------------------------------
+        const bool q8 = !isq && (!isv || a.c.v_mode != G9_V_COPY16);
+        if (!__any_sync(0xffffffffu, live && !isq && stored)) continue;
+        uint16_t scale;
+        const uint2 qw = quant8(v, scale);
+        const int h = isv ? r - a.Hq - a.Hkv : r - a.Hq;
+        const bool put = live && stored && !isq;
+        const bool rows8 = q8 && !(isv && a.c.v_mode == G9_V_Q8T);
+        uint8_t* dst = nullptr;
+        if (put)
+          dst = isv ? a.c.v + blk * a.c.v_page_stride + off * a.c.v_tok_stride + h * a.c.v_head_stride
+                    : a.c.k + blk * a.c.k_page_stride + off * a.c.k_tok_stride + h * a.c.k_head_stride;
+        write_q8_row(dst, qw, scale, hl, put && rows8, isv ? a.v_w8 : a.k_w8, stage);
+        if (put && isv && a.c.v_mode == G9_V_COPY16) {
+          store8(dst, 8 * hl, a.v_dt, a.v_w16, v, raw[x].a);
+        } else if (put && isv && a.c.v_mode == G9_V_Q8T) {
+          uint8_t* rec = a.c.v + blk * a.c.v_page_stride + h * a.c.v_head_stride;
+          const int bs = a.c.block_size;
+          if ((hl & 3) == 0) *reinterpret_cast<uint16_t*>(rec + 2 * ((int64_t)(hl >> 2) * bs + off)) = scale;
+          uint8_t* o = rec + 2 * (D / QK) * bs + (int64_t)8 * hl * bs + off;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) o[(int64_t)e * bs] = (uint8_t)((e < 4 ? qw.x : qw.y) >> (8 * (e & 3)));
+        }
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// read_kv: rows of the cache by slot, as 16- or 32-bit values
+// ---------------------------------------------------------------------------
+struct ReadArgs {
+  G9KvCache c;
+  const int64_t* slots;
+  int N, Hkv, out_dt, v_src;                       // v_src: DT_F16 / DT_BF16 of 16-bit V rows
+  void* k_out; void* v_out;                        // [N, Hkv, 128]; v_out may be null
+};
+
+__device__ __forceinline__ void q8_lane(const uint8_t* row, int hl, float v[8]) {
+  const uint8_t* b = row + (hl >> 2) * QBLOCK;
+  const float d = __half2float(__ushort_as_half(*reinterpret_cast<const uint16_t*>(b)));
+  const uint16_t* q = reinterpret_cast<const uint16_t*>(b + 2 + 8 * (hl & 3));
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint16_t w = q[e];
+    v[2 * e] = (float)(int8_t)(w & 0xff) * d;
+    v[2 * e + 1] = (float)(int8_t)(w >> 8) * d;
+  }
+}
+
+__global__ void __launch_bounds__(ns::WARPS * 32) read_kv_kernel(const __grid_constant__ ReadArgs a) {
+  using namespace ns;
+  const int hl = threadIdx.x & 15;
+  const int64_t rows = (int64_t)a.N * a.Hkv;
+  const int64_t step = (int64_t)gridDim.x * WARPS * 2;
+  for (int64_t r = (int64_t)blockIdx.x * WARPS * 2 + (threadIdx.x >> 4); r < rows; r += step) {
+    const int64_t n = r / a.Hkv;
+    const int h = (int)(r - n * a.Hkv);
+    const int64_t slot = a.slots[n];
+    float k[8], v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) k[e] = v[e] = 0.f;
+    const int64_t blk = slot / a.c.block_size;
+    const int off = (int)(slot - blk * a.c.block_size);
+    const bool bad = slot >= 0 && a.c.num_blocks > 0 && blk >= a.c.num_blocks;
+    if (bad) raise_error(ERR_BAD_INDEX);
+    if (slot >= 0 && !bad) {
+      q8_lane(a.c.k + blk * a.c.k_page_stride + off * a.c.k_tok_stride + h * a.c.k_head_stride, hl, k);
+      if (a.v_out) {
+        if (a.c.v_mode == G9_V_Q8T) {
+          const uint8_t* rec = a.c.v + blk * a.c.v_page_stride + h * a.c.v_head_stride;
+          const int bs = a.c.block_size;
+          const float d = __half2float(__ushort_as_half(
+              *reinterpret_cast<const uint16_t*>(rec + 2 * ((int64_t)(hl >> 2) * bs + off))));
+          const int8_t* q = reinterpret_cast<const int8_t*>(rec + 2 * (D / QK) * bs + (int64_t)8 * hl * bs + off);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = (float)q[(int64_t)e * bs] * d;
+        } else {
+          const uint8_t* row = a.c.v + blk * a.c.v_page_stride + off * a.c.v_tok_stride + h * a.c.v_head_stride;
+          if (a.c.v_mode == G9_V_Q8) q8_lane(row, hl, v);
+          else
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = load_one(row, 8 * hl + e, a.v_src);
+        }
+      }
+    }
+    const uint4 pk = round8(k, a.out_dt);
+    store8(a.k_out, r * D + 8 * hl, a.out_dt, true, k, pk);
+    if (a.v_out) {
+      const uint4 pv = round8(v, a.out_dt);
+      store8(a.v_out, r * D + 8 * hl, a.out_dt, true, v, pv);
+    }
+  }
+}
+
+static int ns_sms() {
+  int dev = 0, sms = 148;
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  return sms;
+}
+
+static bool rows16(const void* base, int dt, int64_t s0, int64_t s1) {
+  const int64_t per = dt == DT_F32 ? 4 : 8;        // elements in 16 bytes
+  return (uintptr_t)base % 16 == 0 && s0 % per == 0 && s1 % per == 0;
+}
+
+// 2-byte aligned Q8_0 rows (scales are 16-bit words), 16-bit V rows likewise
+static bool cache_ok(const G9KvCache& c) {
+  if (!c.k || c.block_size <= 0 || c.num_heads_kv <= 0 || c.num_blocks < 0 || c.v_mode < 0 || c.v_mode > 3) return false;
+  if (((uintptr_t)c.k | (uintptr_t)c.k_page_stride | (uintptr_t)c.k_tok_stride | (uintptr_t)c.k_head_stride) & 1) return false;
+  if (c.v_mode == G9_V_NONE) return true;
+  uintptr_t m = (uintptr_t)c.v | (uintptr_t)c.v_page_stride | (uintptr_t)c.v_head_stride;
+  if (c.v_mode != G9_V_Q8T) m |= (uintptr_t)c.v_tok_stride;
+  return c.v && !(m & 1);
+}
+
+static bool aligned(uintptr_t base, int64_t a, int64_t b, int64_t c, uintptr_t to) {
+  return ((base | (uintptr_t)a | (uintptr_t)b | (uintptr_t)c) & (to - 1)) == 0;
+}
+
+}  // namespace g9
+
+G9_ERROR_ACCESSORS(norm_store)
+
+using namespace g9;
+
+extern "C" cudaError_t gfx906_fa_norm_rope_store_kv(
+    const void* query, int query_dtype, int64_t query_token_stride, int64_t query_head_stride, int num_heads_q,
+    const void* key, int key_dtype, int64_t key_token_stride, int64_t key_head_stride, const void* value,
+    int value_dtype, int64_t value_token_stride, int64_t value_head_stride, const void* q_weight, int q_weight_dtype,
+    const void* k_weight, int k_weight_dtype, float eps, const int64_t* positions, const void* cos_sin_cache,
+    int cos_sin_dtype, int rot_dim, int64_t max_position, int is_neox, const int64_t* slot_mapping,
+    const G9KvCache* cache, void* query_out, int64_t query_out_token_stride, int64_t query_out_head_stride,
+    void* key_out, int64_t key_out_token_stride, int64_t key_out_head_stride, int num_tokens, cudaStream_t stream) {
+  if (!cache || num_tokens < 0 || !cache_ok(*cache)) return cudaErrorInvalidValue;
+  if (!key || !positions || !cos_sin_cache || !slot_mapping || max_position <= 0) return cudaErrorInvalidValue;
+  if (rot_dim <= 0 || rot_dim > 128 || rot_dim % 16) return cudaErrorInvalidValue;
+  auto dt_ok = [](int d) { return d >= 0 && d <= 2; };
+  if (!dt_ok(key_dtype) || !dt_ok(cos_sin_dtype) || !dt_ok(q_weight_dtype) || !dt_ok(k_weight_dtype)) return cudaErrorInvalidValue;
+  if (query && (num_heads_q <= 0 || !dt_ok(query_dtype) || !query_out)) return cudaErrorInvalidValue;
+  if (cache->v_mode != G9_V_NONE && (!value || !dt_ok(value_dtype))) return cudaErrorInvalidValue;
+  if (cache->v_mode == G9_V_COPY16 && value_dtype == G9_DT_F32) return cudaErrorInvalidValue;
+  if (num_tokens == 0) return cudaSuccess;
+  NormStoreArgs a{};
+  a.q = query; a.q_dt = query_dtype; a.q_tok = query_token_stride; a.q_head = query_head_stride;
+  a.k = key; a.k_dt = key_dtype; a.k_tok = key_token_stride; a.k_head = key_head_stride;
+  a.v = value; a.v_dt = value_dtype; a.v_tok = value_token_stride; a.v_head = value_head_stride;
+  a.q_out = query_out; a.qo_tok = query_out_token_stride; a.qo_head = query_out_head_stride;
+  a.k_out = key_out; a.ko_tok = key_out_token_stride; a.ko_head = key_out_head_stride;
+  a.q_vec = rows16(query, query_dtype, query_token_stride, query_head_stride);
+  a.k_vec = rows16(key, key_dtype, key_token_stride, key_head_stride);
+  a.v_vec = rows16(value, value_dtype, value_token_stride, value_head_stride);
+  a.qo_vec = rows16(query_out, query_dtype, query_out_token_stride, query_out_head_stride);
+  a.ko_vec = rows16(key_out, key_dtype, key_out_token_stride, key_out_head_stride);
+  a.q_w = q_weight; a.qw_dt = q_weight_dtype; a.k_w = k_weight; a.kw_dt = k_weight_dtype; a.eps = eps;
+  a.positions = positions; a.cos_sin = cos_sin_cache; a.cs_dt = cos_sin_dtype; a.rot = rot_dim; a.neox = is_neox ? 1 : 0;
+  a.max_pos = max_position;
+  a.cs_vec = rows16(cos_sin_cache, cos_sin_dtype, rot_dim, rot_dim / 2);
+  a.slots = slot_mapping;
+  a.c = *cache;
+  a.k_w8 = aligned((uintptr_t)cache->k, cache->k_page_stride, cache->k_tok_stride, cache->k_head_stride, 8);
+  a.v_w8 = aligned((uintptr_t)cache->v, cache->v_page_stride, cache->v_tok_stride, cache->v_head_stride, 8);
+  a.v_w16 = aligned((uintptr_t)cache->v, cache->v_page_stride, cache->v_tok_stride, cache->v_head_stride, 16);
+  a.T = num_tokens; a.Hq = query ? num_heads_q : 0; a.Hkv = cache->num_heads_kv;
+  a.rows = a.Hq + a.Hkv + (cache->v_mode != G9_V_NONE ? a.Hkv : 0);
+  const int sms = ns_sms();
+  // few tokens: a half-warp a row, so that every SM has work; many: BATCH rows share a token's angles and loads overlap
+  a.rpw = (int64_t)num_tokens * a.rows < (int64_t)sms * ns::WARPS * 2 * ns::BATCH ? 1 : ns::BATCH;
+  const int64_t items = (int64_t)num_tokens * ((a.rows + a.rpw - 1) / a.rpw);
+  const int64_t want = (items + ns::WARPS * 2 - 1) / (ns::WARPS * 2);
+  norm_store_kernel<<<(int)(want < (int64_t)sms * 16 ? want : (int64_t)sms * 16), ns::WARPS * 32, 0, stream>>>(a);
+  return cudaGetLastError();
+}
+
+extern "C" cudaError_t gfx906_fa_read_kv(const G9KvCache* cache, int value_dtype, const int64_t* slots, int num_rows,
+                                         void* key_out, void* value_out, int out_dtype, cudaStream_t stream) {
+  if (!cache || num_rows < 0 || !cache_ok(*cache) || out_dtype < 0 || out_dtype > 2) return cudaErrorInvalidValue;
+  if (num_rows == 0) return cudaSuccess;
+  if (!slots || !key_out || (uintptr_t)key_out % 16 || (uintptr_t)value_out % 16) return cudaErrorInvalidValue;
+  if (value_out && cache->v_mode == G9_V_NONE) return cudaErrorInvalidValue;
+  if (value_out && cache->v_mode == G9_V_COPY16 && value_dtype != G9_DT_F16 && value_dtype != G9_DT_BF16)
+    return cudaErrorInvalidValue;
+  ReadArgs a{*cache, slots, num_rows, cache->num_heads_kv, out_dtype, value_dtype, key_out, value_out};
+  const int64_t want = ((int64_t)num_rows * a.Hkv + ns::WARPS * 2 - 1) / (ns::WARPS * 2);
+  const int64_t cap = (int64_t)ns_sms() * 32;
+  read_kv_kernel<<<(int)(want < cap ? want : cap), ns::WARPS * 32, 0, stream>>>(a);
+  return cudaGetLastError();
+}

@@ -631,6 +631,305 @@ torch::Tensor paged_attention(torch::Tensor query, torch::Tensor key_cache_q8, t
   return out;
 }
 
+// ---------------------------------------------------------------------------
+// draft-tree speculation (no reference counterpart)
+// ---------------------------------------------------------------------------
+#define CHECK_SAME(x, y) TORCH_CHECK((x).device() == (y).device(), #x " must be on the device of " #y)
+
+// G9KvCache of one layer's views: K [NB, bs, Hkv, D/32*34] uint8 and V as
+// [NB, bs, Hkv, D] 16-bit, [NB, bs, Hkv, D/32*34] uint8 or page-transposed
+// [NB, Hkv, bs*D/32*34] uint8; any strides with contiguous rows.
+G9KvCache kv_layout(const torch::Tensor& k, const torch::Tensor& v, bool with_v, int64_t D) {
+  CHECK_CUDA(k);
+  TORCH_CHECK(k.dim() == 4 && k.dtype() == torch::kUInt8 && k.size(3) == (D / 32) * 34 && k.stride(3) == 1,
+              "k_cache must be uint8 [NB, bs, Hkv, (D/32)*34] with contiguous rows");
+  TORCH_CHECK(k.size(1) > 0 && k.size(2) > 0, "k_cache must have tokens and heads");
+  G9KvCache c{};
+  c.k = k.data_ptr<uint8_t>();
+  c.k_page_stride = k.stride(0);
+  c.k_tok_stride = k.stride(1);
+  c.k_head_stride = k.stride(2);
+  c.num_blocks = k.size(0);
+  c.block_size = k.size(1);
+  c.num_heads_kv = k.size(2);
+  c.v_mode = G9_V_NONE;
+  if (!with_v) return c;
+  CHECK_CUDA(v);
+  CHECK_SAME(v, k);
+  TORCH_CHECK(v.size(0) == k.size(0), "v_cache blocks mismatch");
+  const int64_t e = v.element_size();
+  if (v.dim() == 3) {
+    TORCH_CHECK(v.dtype() == torch::kUInt8 && v.size(1) == k.size(2) && v.size(2) == k.size(1) * k.size(3) && v.stride(2) == 1,
+                "a 3-D v_cache must be uint8 [NB, Hkv, block_size*(D/32)*34] page-transposed records");
+    c.v_mode = G9_V_Q8T;
+    c.v_head_stride = v.stride(1);
+  } else {
+    TORCH_CHECK(v.dim() == 4 && v.size(1) == k.size(1) && v.size(2) == k.size(2) && v.stride(3) == 1,
+                "v_cache must be [NB, bs, Hkv, row] with contiguous rows");
+    if (v.dtype() == torch::kUInt8) {
+      TORCH_CHECK(v.size(3) == (D / 32) * 34, "Q8_0 v_cache last dim must be (D/32)*34");
+      c.v_mode = G9_V_Q8;
+    } else {
+      TORCH_CHECK((v.dtype() == torch::kFloat16 || v.dtype() == torch::kBFloat16) && v.size(3) == D,
+                  "v_cache must be fp16 or bf16 [NB, bs, Hkv, D], or uint8 (Q8_0)");
+      c.v_mode = G9_V_COPY16;
+    }
+    c.v_tok_stride = v.stride(1) * e;
+    c.v_head_stride = v.stride(2) * e;
+  }
+  c.v = reinterpret_cast<uint8_t*>(v.data_ptr());
+  c.v_page_stride = v.stride(0) * e;
+  return c;
+}
+
+void check_index(const torch::Tensor& x, const char* name, c10::ScalarType dt, int64_t n) {
+  TORCH_CHECK(x.device().is_cuda() && x.scalar_type() == dt && x.dim() == 1 && x.is_contiguous(), name,
+              " must be a contiguous 1-D ", dt, " CUDA tensor");
+  TORCH_CHECK(n < 0 || x.size(0) == n, name, " must have ", n, " entries, got ", x.size(0));
+}
+
+std::vector<torch::Tensor> tree_mask(torch::Tensor parents, torch::Tensor query_start_loc, torch::Tensor seq_lens,
+                                     int64_t max_query_len) {
+  check_index(parents, "parents", torch::kInt32, -1);
+  check_index(query_start_loc, "query_start_loc", torch::kInt32, -1);
+  const int64_t B = query_start_loc.size(0) - 1, T = parents.size(0);
+  TORCH_CHECK(B >= 0, "query_start_loc must be [num_seqs + 1]");
+  check_index(seq_lens, "seq_lens", torch::kInt32, B);
+  CHECK_SAME(query_start_loc, parents);
+  CHECK_SAME(seq_lens, parents);
+  TORCH_CHECK(max_query_len > 0 && max_query_len < (int64_t)1 << 30, "max_query_len must be positive");
+  TORCH_CHECK(T == 0 || B > 0, "tokens without a sequence");
+  const int64_t words = (max_query_len + 31) / 32;
+  c10::cuda::CUDAGuard g(parents.device());
+  auto mask = torch::empty({T, words}, parents.options());
+  auto positions = torch::empty({T}, parents.options().dtype(torch::kInt64));
+  check_status(gfx906_fa_tree_mask(parents.data_ptr<int32_t>(), query_start_loc.data_ptr<int32_t>(),
+                                   seq_lens.data_ptr<int32_t>(), (int)B, (int)T, (int)words, mask.data_ptr<int32_t>(),
+                                   positions.data_ptr<int64_t>(), cur_stream()),
+               "gfx906_fa_tree_mask");
+  return {mask, positions};
+}
+
+void norm_rope_store_kv(c10::optional<torch::Tensor> query, torch::Tensor key, torch::Tensor value,
+                        c10::optional<torch::Tensor> q_weight, c10::optional<torch::Tensor> k_weight, double eps,
+                        torch::Tensor positions, torch::Tensor cos_sin_cache, bool is_neox, torch::Tensor slot_mapping,
+                        torch::Tensor k_cache, torch::Tensor v_cache, int64_t v_mode,
+                        c10::optional<torch::Tensor> query_out, c10::optional<torch::Tensor> key_out) {
+  CHECK_CUDA(key);
+  TORCH_CHECK(key.dim() == 3 && key.stride(2) == 1, "key must be [T, Hkv, D] with contiguous D");
+  const int64_t T = key.size(0), Hkv = key.size(1), D = key.size(2);
+  TORCH_CHECK(D == 128, "head_size must be 128");
+  TORCH_CHECK(v_mode >= 0 && v_mode <= 3, "v_mode must be 0..3");
+  const int kdt = dtype_code(key, "key");
+  TORCH_CHECK(positions.device().is_cuda() && positions.dtype() == torch::kInt64 && positions.dim() == 1 &&
+                  positions.size(0) >= T && positions.is_contiguous(), "positions must be contiguous int64 [>= T]");
+  check_index(slot_mapping, "slot_mapping", torch::kInt64, T);
+  CHECK_CUDA(cos_sin_cache);
+  TORCH_CHECK(cos_sin_cache.dim() == 2 && cos_sin_cache.is_contiguous() && cos_sin_cache.size(0) > 0,
+              "cos_sin_cache must be contiguous [max_pos, rot_dim]");
+  const int64_t rot = cos_sin_cache.size(1);
+  TORCH_CHECK(rot > 0 && rot <= D && rot % 16 == 0, "rot_dim must be a multiple of 16 up to 128, got ", rot);
+  const int csdt = dtype_code(cos_sin_cache, "cos_sin_cache");
+  G9KvCache c = kv_layout(k_cache, v_cache, v_mode != 0, D);
+  TORCH_CHECK(c.v_mode == v_mode, "v_cache does not have the layout of v_mode ", v_mode);
+  TORCH_CHECK(c.num_heads_kv == Hkv, "k_cache Hkv mismatch");
+  int vdt = G9_DT_F16;
+  if (v_mode != 0) {
+    CHECK_CUDA(value);
+    CHECK_SAME(value, key);
+    vdt = dtype_code(value, "value");
+    TORCH_CHECK(value.dim() == 3 && value.size(0) == T && value.size(1) == Hkv && value.size(2) == D && value.stride(2) == 1,
+                "value must be [T, Hkv, D] with contiguous D");
+    TORCH_CHECK(v_mode != 1 || value.dtype() == v_cache.dtype(), "value and v_cache must have the same type (v_mode 1)");
+  }
+  auto weight = [&](const c10::optional<torch::Tensor>& w, const char* name, int& dt) -> const void* {
+    dt = G9_DT_F16;
+    if (!w.has_value()) return nullptr;
+    TORCH_CHECK(w->device() == key.device() && w->dim() == 1 && w->size(0) == D && w->is_contiguous(), name,
+                " must be contiguous [D] on the key's device");
+    dt = dtype_code(*w, name);
+    return w->data_ptr();
+  };
+  int qwdt, kwdt;
+  const void* qw = weight(q_weight, "q_weight", qwdt);
+  const void* kw = weight(k_weight, "k_weight", kwdt);
+  for (const auto* x : {&positions, &slot_mapping, &cos_sin_cache, &k_cache})
+    TORCH_CHECK(x->device() == key.device(), "every tensor must be on the key's device");
+  torch::Tensor q, qo;
+  int qdt = G9_DT_F16;
+  if (query.has_value()) {
+    q = *query;
+    CHECK_CUDA(q);
+    CHECK_SAME(q, key);
+    TORCH_CHECK(q.dim() == 3 && q.size(0) >= T && q.size(1) > 0 && q.size(2) == D && q.stride(2) == 1,
+                "query must be [>= T, Hq, D] with contiguous D");
+    qdt = dtype_code(q, "query");
+    qo = query_out.value_or(q);
+    CHECK_SAME(qo, key);
+    TORCH_CHECK(qo.dim() == 3 && qo.size(0) >= T && qo.size(1) == q.size(1) && qo.size(2) == D && qo.stride(2) == 1 &&
+                    qo.dtype() == q.dtype(), "query_out must be [>= T, Hq, D] of the query's type with contiguous D");
+  }
+  if (key_out.has_value()) {
+    CHECK_SAME(*key_out, key);
+    TORCH_CHECK(key_out->dim() == 3 && key_out->size(0) >= T && key_out->size(1) == Hkv && key_out->size(2) == D &&
+                    key_out->stride(2) == 1 && key_out->dtype() == key.dtype(),
+                "key_out must be [>= T, Hkv, D] of the key's type with contiguous D");
+  }
+  if (T == 0) return;
+  const bool wq = query.has_value(), wk = key_out.has_value();
+  c10::cuda::CUDAGuard g(key.device());
+  check_status(gfx906_fa_norm_rope_store_kv(
+                   wq ? q.data_ptr() : nullptr, qdt, wq ? q.stride(0) : 0, wq ? q.stride(1) : 0, wq ? (int)q.size(1) : 0,
+                   key.data_ptr(), kdt, key.stride(0), key.stride(1), v_mode ? value.data_ptr() : nullptr, vdt,
+                   v_mode ? value.stride(0) : 0, v_mode ? value.stride(1) : 0, qw, qwdt, kw, kwdt, (float)eps,
+                   positions.data_ptr<int64_t>(), cos_sin_cache.data_ptr(), csdt, (int)rot, cos_sin_cache.size(0),
+                   is_neox ? 1 : 0, slot_mapping.data_ptr<int64_t>(), &c, wq ? qo.data_ptr() : nullptr,
+                   wq ? qo.stride(0) : 0, wq ? qo.stride(1) : 0, wk ? key_out->data_ptr() : nullptr,
+                   wk ? key_out->stride(0) : 0, wk ? key_out->stride(1) : 0, (int)T, cur_stream()),
+               "gfx906_fa_norm_rope_store_kv");
+}
+
+std::vector<torch::Tensor> read_kv(torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor slots, at::ScalarType dtype) {
+  check_index(slots, "slots", torch::kInt64, -1);
+  CHECK_SAME(slots, k_cache);
+  const G9KvCache c = kv_layout(k_cache, v_cache, true, 128);
+  const int64_t N = slots.size(0);
+  auto k = torch::empty({N, c.num_heads_kv, 128}, k_cache.options().dtype(dtype));
+  auto v = torch::empty_like(k);
+  const int dt = dtype_code(k, "dtype");
+  c10::cuda::CUDAGuard g(k_cache.device());
+  check_status(gfx906_fa_read_kv(&c, c.v_mode == G9_V_COPY16 ? dtype_code(v_cache, "v_cache") : G9_DT_F16,
+                                 slots.data_ptr<int64_t>(), (int)N, k.data_ptr(), v.data_ptr(), dt, cur_stream()),
+               "gfx906_fa_read_kv");
+  return {k, v};
+}
+
+void move_kv(const std::vector<torch::Tensor>& k_caches, const std::vector<torch::Tensor>& v_caches,
+             torch::Tensor src_slots, torch::Tensor dst_slots, int64_t group_size) {
+  const size_t L = k_caches.size();
+  TORCH_CHECK(v_caches.size() == L || v_caches.empty(), "k_caches and v_caches must have one entry per layer");
+  check_index(src_slots, "src_slots", torch::kInt64, -1);
+  const int64_t N = src_slots.size(0);
+  check_index(dst_slots, "dst_slots", torch::kInt64, N);
+  CHECK_SAME(dst_slots, src_slots);
+  TORCH_CHECK(group_size > 0 && N % group_size == 0, "src_slots must hold whole groups of group_size pairs");
+  if (L == 0 || N == 0) return;
+  const bool with_v = !v_caches.empty();
+  const G9KvCache c = kv_layout(k_caches[0], with_v ? v_caches[0] : k_caches[0], with_v, 128);
+  std::vector<void*> ks(L), vs(with_v ? L : 0);
+  for (size_t i = 0; i < L; ++i) {
+    TORCH_CHECK(k_caches[i].device() == src_slots.device() && k_caches[i].sizes() == k_caches[0].sizes() &&
+                    k_caches[i].strides() == k_caches[0].strides() && k_caches[i].dtype() == k_caches[0].dtype(),
+                "every layer's k_cache must have the layout of the first, on the slots' device");
+    ks[i] = k_caches[i].data_ptr();
+    if (!with_v) continue;
+    TORCH_CHECK(v_caches[i].device() == src_slots.device() && v_caches[i].sizes() == v_caches[0].sizes() &&
+                    v_caches[i].strides() == v_caches[0].strides() && v_caches[i].dtype() == v_caches[0].dtype(),
+                "every layer's v_cache must have the layout of the first, on the slots' device");
+    vs[i] = v_caches[i].data_ptr();
+  }
+  c10::cuda::CUDAGuard g(src_slots.device());
+  check_status(gfx906_fa_move_kv(ks.data(), with_v ? vs.data() : nullptr, (int)L, &c, src_slots.data_ptr<int64_t>(),
+                                 dst_slots.data_ptr<int64_t>(), (int)(N / group_size), (int)group_size, cur_stream()),
+               "gfx906_fa_move_kv");
+}
+
+void copy_pages(const std::vector<torch::Tensor>& caches, torch::Tensor src_pages, torch::Tensor dst_pages) {
+  check_index(src_pages, "src_pages", torch::kInt64, -1);
+  check_index(dst_pages, "dst_pages", torch::kInt64, src_pages.size(0));
+  CHECK_SAME(dst_pages, src_pages);
+  if (caches.empty() || src_pages.size(0) == 0) return;
+  const auto& f = caches[0];
+  TORCH_CHECK(f.dim() >= 2 && f.size(0) > 0, "a cache must be [num_blocks, ...]");
+  TORCH_CHECK(f[0].is_contiguous(), "a page must be contiguous");
+  std::vector<void*> at(caches.size());
+  for (size_t i = 0; i < caches.size(); ++i) {
+    const auto& x = caches[i];
+    TORCH_CHECK(x.device().is_cuda() && x.device() == src_pages.device() && x.sizes() == f.sizes() &&
+                    x.strides() == f.strides() && x.dtype() == f.dtype(),
+                "every layer's cache must have the layout of the first, on the pages' device");
+    at[i] = x.data_ptr();
+  }
+  const int64_t e = f.element_size();
+  c10::cuda::CUDAGuard g(src_pages.device());
+  check_status(gfx906_fa_copy_pages(at.data(), (int)at.size(), f.size(0), f.stride(0) * e, f.numel() / f.size(0) * e,
+                                    src_pages.data_ptr<int64_t>(), dst_pages.data_ptr<int64_t>(),
+                                    (int)src_pages.size(0), cur_stream()),
+               "gfx906_fa_copy_pages");
+}
+
+// tree_attention: paged_attention's layout; the last n_q cache rows of each
+// sequence are its drafts, and tree_mask's bit rows say which of them a draft
+// sees (tree_mask [T, words] int32, see gfx906_fa_tree_attention).
+torch::Tensor tree_attention(torch::Tensor query, torch::Tensor key_cache_q8, torch::Tensor value_cache,
+                             torch::Tensor block_table, torch::Tensor seq_lens, torch::Tensor query_start_loc,
+                             torch::Tensor tree_mask, int64_t max_query_len, int64_t max_seq_len, double scale,
+                             c10::optional<torch::Tensor> out_opt, double softcap, int64_t sliding_window,
+                             c10::optional<torch::Tensor> sinks, c10::optional<torch::Tensor> output_scale) {
+  CHECK_CUDA(query);
+  TORCH_CHECK(query.dim() == 3 && query.stride(2) == 1, "query must be [T, Hq, D] with contiguous D");
+  const int qdt = dtype_code(query, "query");
+  const int64_t T = query.size(0), Hq = query.size(1), D = query.size(2), B = block_table.size(0);
+  check_paged(key_cache_q8, value_cache, block_table, seq_lens, D, B);
+  check_index(query_start_loc, "query_start_loc", torch::kInt32, B + 1);
+  TORCH_CHECK(Hq > 0 && key_cache_q8.size(2) > 0 && Hq % key_cache_q8.size(2) == 0, "heads_q must be divisible by heads_kv");
+  TORCH_CHECK(tree_mask.device().is_cuda() && tree_mask.dtype() == torch::kInt32 && tree_mask.dim() == 2 &&
+                  tree_mask.size(0) >= T && (tree_mask.size(1) <= 1 || tree_mask.stride(1) == 1),
+              "tree_mask must be int32 [>= T, words] with contiguous words");
+  TORCH_CHECK(max_query_len >= 0 && tree_mask.size(1) * 32 >= max_query_len,
+              "tree_mask rows must have a bit for every draft of the longest tree (", max_query_len, ")");
+  TORCH_CHECK(max_seq_len >= 0 && max_seq_len <= INT32_MAX && max_query_len <= INT32_MAX, "lengths must fit 32 bits");
+  for (const auto* x : {&key_cache_q8, &value_cache, &block_table, &seq_lens, &query_start_loc, &tree_mask})
+    TORCH_CHECK(x->device() == query.device(), "every tensor must be on the query's device");
+  const int vfmt = infer_v_fmt(value_cache, D);
+  torch::Tensor out;
+  if (out_opt.has_value()) {
+    out = out_opt.value();
+    TORCH_CHECK(out.dim() == 3 && out.size(0) >= T && out.size(1) == Hq && out.size(2) == D && out.stride(2) == 1,
+                "out must be [>=T, Hq, D] with contiguous D");
+    CHECK_SAME(out, query);
+  } else {
+    out = torch::empty({T, Hq, D}, query.options());
+  }
+  if (B == 0 || T == 0 || max_query_len == 0) return out;
+  c10::cuda::CUDAGuard g(query.device());
+  G9AttnBatch b = batch_base(key_cache_q8, value_cache, vfmt, block_table, seq_lens);
+  b.q = query.data_ptr();
+  b.q_dtype = qdt;
+  b.q_tok_stride = query.stride(0);
+  b.q_head_stride = query.stride(1);
+  b.q_start = query_start_loc.data_ptr<int32_t>();
+  b.flags = G9_F_CU_SEQLENS;
+  b.seq_q = (int)std::min<int64_t>(max_query_len, T);
+  b.out = out.data_ptr();
+  torch::Tensor oscale_c, sinks_c;
+  if (out.scalar_type() == torch::kFloat8_e4m3fn) {
+    TORCH_CHECK(output_scale.has_value(), "an fp8 (e4m3) out needs output_scale");
+    oscale_c = output_scale.value().to(torch::kFloat32).reshape({-1}).contiguous();
+    TORCH_CHECK(oscale_c.numel() == 1 && oscale_c.device() == query.device(),
+                "output_scale must be one fp32 value on the query's device");
+    b.out_dtype = G9_DT_FP8E4M3;
+    b.out_scale = oscale_c.data_ptr<float>();
+  } else {
+    TORCH_CHECK(!output_scale.has_value(), "output_scale applies to an fp8 (e4m3) out only");
+    b.out_dtype = dtype_code(out, "out");
+  }
+  b.o_tok_stride = out.stride(0);
+  b.o_head_stride = out.stride(1);
+  b.max_kv = (int)max_seq_len;
+  b.num_heads_q = Hq;
+  b.head_dim = D;
+  b.scale = (float)scale;
+  set_features(b, Hq, softcap, sliding_window, sinks, sinks_c, query);
+  const size_t ws = gfx906_fa_tree_attention_workspace_size(&b);
+  torch::Tensor wsbuf;
+  if (ws) wsbuf = torch::empty({(int64_t)ws}, query.options().dtype(torch::kUInt8));
+  check_status(gfx906_fa_tree_attention(&b, tree_mask.data_ptr<int32_t>(), tree_mask.stride(0), (int)tree_mask.size(1),
+                                        ws ? wsbuf.data_ptr() : nullptr, ws, cur_stream()),
+               "gfx906_fa_tree_attention");
+  return out;
+}
+
 unsigned int device_error(bool clear) {
   unsigned int v = 0;
   check_status(gfx906_fa_get_device_error(&v), "gfx906_fa_get_device_error");
@@ -678,6 +977,29 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("seq_lens"), py::arg("query_start_loc"), py::arg("max_query_len"), py::arg("max_seq_len"),
         py::arg("scale"), py::arg("out") = c10::nullopt, py::arg("query_lens_host") = c10::nullopt,
         py::arg("seq_lens_host") = c10::nullopt, py::arg("softcap") = 0.0, py::arg("sliding_window") = 0,
+        py::arg("sinks") = c10::nullopt, py::arg("output_scale") = c10::nullopt);
+  m.def("tree_mask", &tree_mask,
+        "Ancestor bit rows int32 [T, ceil(max_query_len/32)] and positions int64 [T] of drafted token trees from their "
+        "parent links",
+        py::arg("parents"), py::arg("query_start_loc"), py::arg("seq_lens"), py::arg("max_query_len"));
+  m.def("norm_rope_store_kv", &norm_rope_store_kv,
+        "Per-head RMS norm + RoPE of query (into query_out, default in place) and key, K -> Q8_0, V per v_mode, by "
+        "slot_mapping; the rotated key is written only to key_out",
+        py::arg("query"), py::arg("key"), py::arg("value"), py::arg("q_weight"), py::arg("k_weight"), py::arg("eps"),
+        py::arg("positions"), py::arg("cos_sin_cache"), py::arg("is_neox"), py::arg("slot_mapping"), py::arg("k_cache"),
+        py::arg("v_cache"), py::arg("v_mode") = 1, py::arg("query_out") = c10::nullopt, py::arg("key_out") = c10::nullopt);
+  m.def("read_kv", &read_kv, "Cache rows by slot as values: [k, v], each [N, Hkv, D] of dtype (slot < 0: zeros)",
+        py::arg("k_cache"), py::arg("v_cache"), py::arg("slots"), py::arg("dtype"));
+  m.def("move_kv", &move_kv,
+        "Move cache rows src_slots -> dst_slots in every layer, whole groups of group_size pairs at once",
+        py::arg("k_caches"), py::arg("v_caches"), py::arg("src_slots"), py::arg("dst_slots"), py::arg("group_size"));
+  m.def("copy_pages", &copy_pages, "Copy whole pages src_pages -> dst_pages in every layer", py::arg("caches"),
+        py::arg("src_pages"), py::arg("dst_pages"));
+  m.def("tree_attention", &tree_attention,
+        "Attention of drafted token trees over the paged cache: query [T, Hq, D] -> out [T, Hq, D]",
+        py::arg("query"), py::arg("key_cache_q8"), py::arg("value_cache"), py::arg("block_table"), py::arg("seq_lens"),
+        py::arg("query_start_loc"), py::arg("tree_mask"), py::arg("max_query_len"), py::arg("max_seq_len"),
+        py::arg("scale"), py::arg("out") = c10::nullopt, py::arg("softcap") = 0.0, py::arg("sliding_window") = 0,
         py::arg("sinks") = c10::nullopt, py::arg("output_scale") = c10::nullopt);
   m.def("device_error", &device_error, "Read (and optionally clear) the library's device error word",
         py::arg("clear") = false);

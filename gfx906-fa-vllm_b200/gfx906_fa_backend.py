@@ -81,6 +81,9 @@ class Gfx906FAMetadata:
     # exact query lengths and upper bounds of the context lengths
     query_lens_host: list | None = field(default=None)
     seq_lens_host: list | None = field(default=None)
+    # draft-tree speculation: gfx906_fa.tree_mask's bit rows of this step's
+    # query tokens, set by the caller that drafted them (None: causal)
+    tree_mask: torch.Tensor | None = field(default=None)
 
 
 class Gfx906FAMetadataBuilder(AttentionMetadataBuilder[Gfx906FAMetadata]):
@@ -303,6 +306,8 @@ class Gfx906FAImpl(AttentionImpl):
         q = query[:n]
         out = output[:n].view(n, self.num_heads, self.head_size)
         if self._legacy:
+            if attn_metadata.tree_mask is not None:
+                raise NotImplementedError("GFX906_FA: draft trees need the Q8_0 cache path (GFX906_FA_LEGACY=0)")
             key_cache, value_cache = kv_cache.unbind(1)
             res = forward_paged(q, key_cache, value_cache, attn_metadata.block_table, attn_metadata.seq_lens,
                                 attn_metadata.query_start_loc, attn_metadata.max_query_len,
@@ -317,7 +322,7 @@ class Gfx906FAImpl(AttentionImpl):
                       scale=self.scale, key_cache_q8=k_q8, out=out,
                       query_lens_host=attn_metadata.query_lens_host, seq_lens_host=attn_metadata.seq_lens_host,
                       softcap=self.logits_soft_cap, sliding_window=self.sliding_window, sinks=self._sinks_f32(),
-                      output_scale=output_scale)
+                      output_scale=output_scale, tree_mask=attn_metadata.tree_mask)
         return output
 
     def _sinks_f32(self):

@@ -137,6 +137,7 @@ def forward_paged(
     sliding_window: int = 0,
     sinks: Optional[torch.Tensor] = None,
     output_scale: Optional[torch.Tensor] = None,
+    tree_mask: Optional[torch.Tensor] = None,
 ) -> torch.Tensor:
     """vLLM-layout paged attention (reference: gfx906_fa_paged.py:197-465).
 
@@ -152,7 +153,10 @@ def forward_paged(
     qp - k < sliding_window) and `sinks` ([Hq] logits added to each softmax
     denominator), on every path; `output_scale` with an fp8 (e4m3) `out`:
     vLLM's static per-tensor output quantisation, out = e4m3(o / scale)
-    (direct path)."""
+    (direct path); `tree_mask` (`gfx906_fa.tree_mask`'s bit rows, [num_tokens,
+    words] int32): the query tokens of each sequence are a draft tree, its
+    last cache rows, and see their context and their own ancestors instead of
+    the causal rule (needs key_cache_q8; always the direct path)."""
     num_tokens, Hq, D = query.shape
     num_seqs = block_table.shape[0]
     if scale is None:
@@ -162,6 +166,15 @@ def forward_paged(
     bt, sl = bt.contiguous(), sl.contiguous()
     cu = cu_seqlens_q if cu_seqlens_q.dtype == torch.int32 else cu_seqlens_q.to(torch.int32)
     cu = cu.contiguous()
+
+    if tree_mask is not None:
+        if key_cache_q8 is None:
+            raise NotImplementedError("draft trees need the Q8_0 key cache (key_cache_q8)")
+        o = out if out is not None else torch.empty((num_tokens, Hq, D), dtype=torch.float32, device=query.device)
+        gfx906_fa.tree_attention(query, key_cache_q8, value_cache, bt, sl, cu, tree_mask, int(max_seqlen_q),
+                                 int(max_seqlen_k), float(scale), out=o, softcap=float(softcap),
+                                 sliding_window=int(sliding_window), sinks=sinks, output_scale=output_scale)
+        return o if out is not None else o.view(num_tokens, Hq * D)
 
     # page-transposed Q8_0 V is only read by the direct kernels
     v_q8t = value_cache is not None and value_cache.dim() == 3

@@ -320,8 +320,104 @@ cudaError_t gfx906_fa_launch_paged(const float* Q_fp32, const void* K_paged, con
                                    int64_t k_token_stride, int64_t k_head_stride, int64_t v_block_stride,
                                    int64_t v_token_stride, int64_t v_head_stride, float scale, cudaStream_t stream);
 
+/* ----------------------------------------------------------------------- */
+/* Draft-tree speculation (no reference counterpart: its attention is causal) */
+/* ----------------------------------------------------------------------- */
+
+/* One layer's paged KV cache, byte strides.  K rows are Q8_0; V per v_mode:
+ * G9_V_COPY16 16-bit rows, G9_V_Q8 Q8_0 token rows, G9_V_Q8T page-transposed
+ * records (v_tok_stride unused), G9_V_NONE absent.  A slot is
+ * page * block_size + offset; head size 128. */
+typedef struct G9KvCache {
+  uint8_t* k;
+  int64_t k_page_stride, k_tok_stride, k_head_stride;
+  uint8_t* v;
+  int64_t v_page_stride, v_tok_stride, v_head_stride;
+  int v_mode;
+  int num_blocks; /* slots at or past num_blocks * block_size are skipped and set bit 3 of the error word */
+  int block_size;
+  int num_heads_kv;
+} G9KvCache;
+
+/* Ancestor bit rows and positions of drafted token trees.  Sequence b drafted
+ * tokens query_start_loc[b] .. query_start_loc[b+1]-1; parents[t] is the index
+ * of token t's parent among its sequence's drafts (smaller than t's own), or
+ * negative for a token that follows the context.  mask [num_tokens,
+ * mask_words]: bit j%32 of word j/32 of row t is 1 iff draft j is token t or
+ * one of its ancestors.  positions (int64 [num_tokens], optional) =
+ * seq_lens[b] - n_b + depth, seq_lens counting the drafts.  A link that does
+ * not point to an earlier draft sets bit 3 of the error word and counts as
+ * the context.  Tokens past query_start_loc[num_seqs] get zeros. */
+cudaError_t gfx906_fa_tree_mask(const int32_t* parents, const int32_t* query_start_loc, const int32_t* seq_lens,
+                                int num_seqs, int num_tokens, int mask_words, int32_t* mask, int64_t* positions,
+                                cudaStream_t stream);
+
+/* Per-head RMS norm and rotation of queries and keys, and the KV store, in
+ * one pass: y = x * rsqrt(mean(x^2) + eps) * weight over the 128 elements of a
+ * head (weight [128]; NULL: no norm), rotated by the token's position as in
+ * gfx906_fa_rope_store_kv (rot_dim a multiple of 16 up to 128), in fp32 with
+ * one rounding to the tensor's type.  Queries go to query_out (may be the
+ * query; query NULL: keys only), keys to key_out when it is not NULL (may be
+ * the key); the rounded key is quantised into the cache and V stored per
+ * cache->v_mode by slot_mapping (slot < 0: not stored).  A position outside
+ * 0 .. max_position-1 (the rows of cos_sin_cache) sets bit 3 of the error
+ * word and reads row 0. */
+cudaError_t gfx906_fa_norm_rope_store_kv(
+    const void* query, int query_dtype, int64_t query_token_stride, int64_t query_head_stride, int num_heads_q,
+    const void* key, int key_dtype, int64_t key_token_stride, int64_t key_head_stride, const void* value,
+    int value_dtype, int64_t value_token_stride, int64_t value_head_stride, const void* q_weight, int q_weight_dtype,
+    const void* k_weight, int k_weight_dtype, float eps, const int64_t* positions, const void* cos_sin_cache,
+    int cos_sin_dtype, int rot_dim, int64_t max_position, int is_neox, const int64_t* slot_mapping,
+    const G9KvCache* cache, void* query_out, int64_t query_out_token_stride, int64_t query_out_head_stride,
+    void* key_out, int64_t key_out_token_stride, int64_t key_out_head_stride, int num_tokens, cudaStream_t stream);
+
+/* Rows of the cache by slot, as values: key_out / value_out [num_rows, Hkv,
+ * 128] contiguous, 16-byte aligned, of out_dtype (F16 / BF16 / F32); value_out
+ * may be NULL.  value_dtype: type of 16-bit V rows.  A slot < 0 gives zeros. */
+cudaError_t gfx906_fa_read_kv(const G9KvCache* cache, int value_dtype, const int64_t* slots, int num_rows,
+                              void* key_out, void* value_out, int out_dtype, cudaStream_t stream);
+
+/* Moves cache rows src_slots[i] -> dst_slots[i] in every layer (k_layers /
+ * v_layers: host arrays of device addresses; strides, mode and sizes from
+ * *cache, whose k and v are not used).  Pairs come in num_groups groups of
+ * group_size and move as if all rows of a group were read before any is
+ * written; different groups must not share slots, and no destination may
+ * appear twice.  A pair with a negative slot is skipped.  group_size *
+ * (136 + bytes of a V row) must fit 96 KB less 16 bytes a pair. */
+cudaError_t gfx906_fa_move_kv(void* const* k_layers, void* const* v_layers, int num_layers, const G9KvCache* cache,
+                              const int64_t* src_slots, const int64_t* dst_slots, int num_groups, int group_size,
+                              cudaStream_t stream);
+
+/* Copies whole pages src_pages[i] -> dst_pages[i] (page_bytes at
+ * page * page_stride) in every layer.  A negative entry skips the pair, one at
+ * or past num_blocks skips it and sets bit 1 of the error word.  No
+ * destination may also be a source or appear twice. */
+cudaError_t gfx906_fa_copy_pages(void* const* layers, int num_layers, int64_t num_blocks, int64_t page_stride,
+                                 int64_t page_bytes, const int64_t* src_pages, const int64_t* dst_pages,
+                                 int num_pairs, cudaStream_t stream);
+
+/* Attention of drafted token trees over the paged cache.  The batch is
+ * described as for gfx906_fa_attention, without q_abs and mask; sequence b's
+ * n_q drafts are its last n_q cache rows (kv_len counts them).  With
+ * ctx = kv_len[b] - n_q[b], query token t sees every context key k < ctx and
+ * draft j (key ctx + j) iff bit j of its row is 1: row q_start[b] + t of
+ * tree_mask (mask_words int32 a row, mask_row_stride int32 apart), or row
+ * b * seq_q + t without q_start.  Draft keys past mask_words * 32 are hidden.
+ * window > 0: a context key k is visible iff
+ * ctx + (visible drafts - 1) - k < window, the distance along the token's own
+ * path; drafts are governed by their bits alone.  A row that sees nothing is
+ * written as zeros; a key no row's bits select never reaches that row, whatever its
+ * cache row holds.  softcap, sinks, num_blocks, flags
+ * (G9_F_CU_SEQLENS) and fp8 output as in gfx906_fa_attention.  workspace: at
+ * least gfx906_fa_tree_attention_workspace_size() bytes (which may be 0),
+ * 16-byte aligned, contents need no initialisation. */
+size_t gfx906_fa_tree_attention_workspace_size(const G9AttnBatch* batch);
+cudaError_t gfx906_fa_tree_attention(const G9AttnBatch* batch, const int32_t* tree_mask, int64_t mask_row_stride,
+                                     int mask_words, void* workspace, size_t workspace_bytes, cudaStream_t stream);
+
 /* Device error word (bit 0: a bounded wait timed out, bit 1: a block-table
- * entry was out of range, bit 2: tensor-memory allocation failed).
+ * entry was out of range, bit 2: tensor-memory allocation failed, bit 3: a
+ * slot, position or parent link was out of range).
  * gfx906_fa_get_device_error synchronises the current device and reads it;
  * gfx906_fa_clear_device_error resets it to zero. */
 cudaError_t gfx906_fa_get_device_error(unsigned int* out);
