@@ -6,7 +6,8 @@
 // (no relocatable device code); the C ABI ORs them together.
 #define G9_ERROR_UNITS(X) \
   X(store) X(gather) X(prefill) X(capi) X(decode_v0) X(decode_v0g) X(decode_v1) X(decode_v1g) X(decode_v2) \
-  X(decode_v2g) X(decode_v3) X(decode_v3g) X(tree_mask) X(norm_store) X(kv_move) X(tree_rows)
+  X(decode_v2g) X(decode_v3) X(decode_v3g) X(tree_mask) X(norm_store) X(kv_move) X(tree_rows) \
+  X(tree_v0) X(tree_v1) X(tree_v2) X(tree_v3)
 
 namespace g9 {
 #define G9_DECLARE(tag)                      \

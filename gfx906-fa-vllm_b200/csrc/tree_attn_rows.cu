@@ -1,5 +1,7 @@
-// tree_attn_rows.cu -- attention of drafted token trees, any cache strides
-// and page size.
+// tree_attn_rows.cu -- entry points of the draft-tree attention, and its
+// kernel for caches the tensor-core kernels (tree_attn_tc.cuh) cannot read:
+// pages that are not a multiple of 16 tokens, or rows off the 8-byte (Q8_0)
+// or 16-byte (16-bit V, page-transposed V) boundaries that their copies need.
 //
 //   o_t = sum_k p_tk v_k,  p = softmax over the keys token t sees:
 //   context keys k < ctx (inside its window) and the drafts its bit row selects
@@ -7,7 +9,9 @@
 // A warp per (token, query head): lane k of a 32-key step scores key k, the
 // running maximum and sum are kept in fp32, and lane l accumulates output
 // elements 4l .. 4l+3.
-#include "tree_common.cuh"
+#include <algorithm>
+
+#include "tree_attn_tc.cuh"
 
 namespace g9 {
 
@@ -150,16 +154,60 @@ static bool tree_batch_ok(const G9AttnBatch& p) {
   return !(v & 1) && o % (2 * es) == 0;
 }
 
+namespace g9 {
+cudaError_t launch_tree_tc_v0(const TreeTcParams& pp, int nq, cudaStream_t stream);
+cudaError_t launch_tree_tc_v1(const TreeTcParams& pp, int nq, cudaStream_t stream);
+cudaError_t launch_tree_tc_v2(const TreeTcParams& pp, int nq, cudaStream_t stream);
+cudaError_t launch_tree_tc_v3(const TreeTcParams& pp, int nq, cudaStream_t stream);
+}  // namespace g9
+
+namespace {
+
+struct TreePlan {
+  int nq = 0;                    // query tiles a CTA holds; 0: the row kernel
+  int NG = 0, rc = 0;
+  size_t cum = 0, po = 0, total = 0;
+};
+
+TreePlan plan_tree(const G9AttnBatch& p) {
+  TreePlan pl;
+  auto off = [](uintptr_t base, int64_t a, int64_t b, int64_t c, uintptr_t to) {
+    return ((base | (uintptr_t)a | (uintptr_t)b | (uintptr_t)c) & (to - 1)) != 0;
+  };
+  if (p.block_size % 16) return pl;
+  if (off((uintptr_t)p.k_cache, p.k_page_stride, p.k_tok_stride, p.k_head_stride, 8)) return pl;
+  const uintptr_t va = p.v_fmt == G9_VFMT_Q8 ? 8 : 16;
+  if (off((uintptr_t)p.v_cache, p.v_page_stride, p.v_fmt == G9_VFMT_Q8T ? 0 : p.v_tok_stride, p.v_head_stride, va)) return pl;
+  const int64_t lim = 1 << 26;               // 16 rows' offsets are held in 32 bits
+  if (std::abs(p.k_tok_stride) >= lim || std::abs(p.v_tok_stride) >= lim || p.block_size >= (1 << 20)) return pl;
+  const int64_t rows = (int64_t)p.seq_q * (p.num_heads_q / p.num_heads_kv);
+  const int nq = rows > tt::BM ? 2 : 1;
+  const int64_t groups = (rows + nq * tt::BM - 1) / (nq * tt::BM);
+  const int64_t units = (int64_t)p.num_seqs * groups * ((int64_t)p.max_kv / tt::BN + 1);
+  if (units > 0x3fffffff || (int64_t)p.num_seqs * groups * 8 > 0x7fffffff || p.num_heads_kv > 65535) return pl;
+  int dev = 0, sms = 148;
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  pl.nq = nq;
+  pl.NG = (int)std::max<int64_t>(1, std::min<int64_t>(sms / p.num_heads_kv, units));
+  pl.rc = (int)std::min<int64_t>(nq * tt::BM, (rows + 31) / 32 * 32);
+  auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
+  const size_t slots = (size_t)2 * pl.NG * p.num_heads_kv;
+  pl.cum = up(((size_t)p.num_seqs + 1) * sizeof(int));
+  pl.po = up(slots * tt::D * pl.rc * sizeof(float));
+  pl.total = pl.cum + pl.po + up(slots * 2 * pl.rc * sizeof(float)) + 256;
+  return pl;
+}
+
+}  // namespace
+
 extern "C" size_t gfx906_fa_tree_attention_workspace_size(const G9AttnBatch* batch) {
-  (void)batch;
-  return 0;
+  if (!batch || !tree_batch_ok(*batch) || batch->num_seqs == 0 || batch->seq_q == 0) return 0;
+  return plan_tree(*batch).total;
 }
 
 extern "C" cudaError_t gfx906_fa_tree_attention(const G9AttnBatch* batch, const int32_t* tree_mask,
                                                 int64_t mask_row_stride, int mask_words, void* workspace,
                                                 size_t workspace_bytes, cudaStream_t stream) {
-  (void)workspace;
-  (void)workspace_bytes;
   if (!batch || !tree_batch_ok(*batch) || mask_words <= 0) return cudaErrorInvalidValue;
   if (batch->num_seqs == 0 || batch->seq_q == 0) return cudaSuccess;
   if (!tree_mask || !batch->q || !batch->out || !batch->k_cache || !batch->v_cache || !batch->block_table || !batch->kv_len)
@@ -175,5 +223,25 @@ extern "C" cudaError_t gfx906_fa_tree_attention(const G9AttnBatch* batch, const 
     a.cap_in = batch->scale / batch->softcap;
     a.cap_out = batch->softcap * kLog2e;
   }
-  return run_tree_rows(a, stream);
+  const TreePlan pl = plan_tree(*batch);
+  if (pl.nq == 0) return run_tree_rows(a, stream);
+  if (!workspace || workspace_bytes < pl.total) return cudaErrorInvalidValue;
+  TreeTcParams pp{};
+  pp.a = a;
+  pp.Hkv = batch->num_heads_kv;
+  pp.NG = pl.NG;
+  pp.rc = pl.rc;
+  const int64_t es = batch->out_dtype == DT_F32 ? 4 : batch->out_dtype == DT_FP8 ? 1 : 2;
+  pp.out_vec = (((uintptr_t)batch->out | (uintptr_t)(batch->o_seq_stride * es) | (uintptr_t)(batch->o_tok_stride * es) |
+                 (uintptr_t)(batch->o_head_stride * es)) & 15) == 0;
+  uint8_t* w = reinterpret_cast<uint8_t*>(((uintptr_t)workspace + 255) & ~(uintptr_t)255);
+  pp.cum = reinterpret_cast<int*>(w);
+  pp.po = reinterpret_cast<float*>(w + pl.cum);
+  pp.pml = reinterpret_cast<float*>(w + pl.cum + pl.po);
+  switch (batch->v_fmt) {
+    case G9_VFMT_F16: return launch_tree_tc_v0(pp, pl.nq, stream);
+    case G9_VFMT_BF16: return launch_tree_tc_v1(pp, pl.nq, stream);
+    case G9_VFMT_Q8: return launch_tree_tc_v2(pp, pl.nq, stream);
+    default: return launch_tree_tc_v3(pp, pl.nq, stream);
+  }
 }

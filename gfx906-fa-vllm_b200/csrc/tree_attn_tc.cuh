@@ -1,0 +1,1049 @@
+// tree_attn_tc.cuh -- attention of drafted token trees on 5th-generation
+// tensor cores, straight from the paged Q8_0 cache.
+//
+//   S = Q K^T,  P = 2^(S - m) on the keys a row sees,  O += P V,  out = O / l
+//
+// The rows of one kv head of one sequence are its drafts times the GQA group
+// (row = t * G + g): 16 drafts at GQA 6 are 96 rows, so one pass over the cache
+// carries 4 * 96 FLOP per cached byte and the pass is bound by HBM and by the
+// issue slots of dequantisation and softmax together, where a warp-level MMA
+// would be bound by its own rate and a dequantised staging copy by traffic.
+//
+// Work: the key tiles (128 keys) of all (sequence, row group) items laid end
+// to end are cut into NG equal ranges; CTA (g, h) computes range g for kv head
+// h, so the heads of a group walk the same pages at the same time (a K page
+// holds all heads' 136-byte rows, which share memory lines) and every CTA gets
+// the same number of tiles whatever the lengths.  An item cut by a range border
+// leaves partial rows that tree_combine_kernel joins.
+//
+// CTA, 512 threads:
+//   warp 0       issues every tcgen05.mma from one thread
+//   warps 2-3    bring the row tile(s) of Q into shared memory (fp16)
+//   warps 4-7    load cache rows (cp.async, raw) and convert: K to [key][d], V to
+//                [d][key] (page-transposed Q8_0) or [key][d] (token rows); a warp owns 32 keys of
+//                a tile, so loading and converting need no barrier between warps
+//   warps 8-15   two softmax streams, a thread a row (row = TMEM lane)
+// One query tile (NQ = 1): the streams take alternate key tiles of the same
+// rows, each with its own running maximum, sum and accumulator, so that one
+// stream's softmax runs under the other's MMAs; they are joined through TMEM at
+// the end.  NQ = 2 (more than 128 rows): the streams take one row tile each and share
+// every converted key tile.
+// Tensor memory: S0 S1 O0 O1, 128 columns each; P_i over the first half of S_i.
+// Every mbarrier wait is bounded.
+#pragma once
+
+#include "tcgen05.cuh"
+#include "tree_common.cuh"
+
+namespace g9 {
+
+namespace tt {
+constexpr int D = 128;
+constexpr int BM = 128;
+constexpr int BN = 128;
+constexpr int ST = 2;                        // K and V stages
+constexpr int TILE = BM * D * 2;             // 32 KB
+constexpr int NT = 512;
+constexpr int RAW = 32 * (D / QK) * QBLOCK;  // a warp's 32 raw rows: 4352 bytes
+// launch 512 x 128 registers = 128*REG_CTRL + 128*REG_LOAD + 256*REG_SOFT
+constexpr int REG_CTRL = 56;
+constexpr int REG_LOAD = 128;                // as launched
+constexpr int REG_SOFT = 160;
+static_assert(128 * REG_CTRL + 128 * REG_LOAD + 256 * REG_SOFT <= NT * 128, "register split exceeds the launch budget");
+constexpr float kRescale = 8.0f;             // log2 units
+
+// raw slots a warp rotates through, in shared memory left over by the tiles
+constexpr int raw_slots(int nq) { return nq == 1 ? 3 : 2; }
+constexpr int smem_raw_off(int nq) { return (2 * ST + nq) * TILE; }
+constexpr int smem_stat_off(int nq) { return smem_raw_off(nq) + raw_slots(nq) * 4 * RAW; }
+constexpr int smem_bar_off(int nq) { return smem_stat_off(nq) + (nq == 1 ? 2 * 2 * BM * 4 : 0); }
+constexpr int smem_bytes(int nq) { return smem_bar_off(nq) + 512; }
+static_assert(smem_bytes(1) <= 232448 && smem_bytes(2) <= 232448, "shared memory");
+}  // namespace tt
+
+struct TreeTcParams {
+  TreeArgs a;
+  int Hkv, NG;
+  int rc;                        // rows of a partial block (a multiple of 32)
+  int out_vec;                   // output rows may be written 16 bytes at a time
+  int* cum;                      // [num_seqs + 1] first unit of each sequence
+  float* po;                     // [2 * NG][Hkv][128][rc] partial O
+  float* pml;                    // [2 * NG][Hkv][2][rc] partial maximum and sum
+};
+
+// Units of a sequence: row groups x key tiles, at least one tile per row group
+// (a group that sees no key still writes its zeros).
+struct TreeShape { int nq, L, ctx, R, groups, j0, tiles; };
+
+template <int NQ>
+__device__ __forceinline__ TreeShape tree_shape(const TreeArgs& a, int b) {
+  TreeShape s;
+  s.nq = tree_nq(a.p, b);
+  s.L = seq_len_kv(a.p, b);
+  s.ctx = s.L - s.nq;
+  s.R = s.nq * a.G;
+  s.groups = (s.R + NQ * tt::BM - 1) / (NQ * tt::BM);
+  // first context key any row's window can hold (a row sees at least no draft: depth -1)
+  const int lo = a.p.window > 0 ? max(0, s.ctx - a.p.window) : 0;
+  s.j0 = lo / tt::BN;
+  s.tiles = max(1, (s.L + tt::BN - 1) / tt::BN - s.j0);
+  return s;
+}
+
+// First unit of CTA group g: never more groups than units, so that every
+// group below the last has one.
+__device__ __forceinline__ int range_start(int total, int NG, int g) {
+  const int ng = min(NG, total);
+  return g >= ng ? total : (int)((int64_t)g * total / ng);
+}
+
+// A run of key tiles of one (sequence, row group) item inside a CTA's range.
+struct TreeSeg {
+  int b, row0, rows;             // first packed row, rows of the group
+  int j, n;                      // first key tile, tiles
+  int part;                      // -1: the whole item; 0: continues an item; 1: starts one that goes on
+  int nq, L, ctx;
+};
+
+template <int NQ>
+struct TreeWalk {
+  int u, end, b, base;
+  __device__ __forceinline__ bool next(const TreeArgs& a, TreeSeg& s) {
+    while (u < end && b < a.p.num_seqs) {
+      const TreeShape x = tree_shape<NQ>(a, b);
+      const int off = u - base;
+      if (off >= x.groups * x.tiles) {
+        base += x.groups * x.tiles;
+        ++b;
+        continue;
+      }
+      const int rg = off / x.tiles, j = off - rg * x.tiles;
+      // rows spread evenly over the sequence's groups, whole warps of 32
+      const int per = ((x.R + x.groups - 1) / x.groups + 31) & ~31;
+      s.b = b;
+      s.row0 = rg * per;
+      s.rows = max(0, min(per, x.R - s.row0));
+      s.j = x.j0 + j;
+      s.n = min(x.tiles - j, end - u);
+      s.part = j > 0 ? 0 : (s.n < x.tiles ? 1 : -1);
+      s.nq = x.nq;
+      s.L = x.L;
+      s.ctx = x.ctx;
+      u += s.n;
+      return true;
+    }
+    return false;
+  }
+};
+
+// Rows a tile of 128 keys starting at k0 must check key by key.
+__device__ __forceinline__ bool tree_checked(const TreeArgs& a, const TreeSeg& s, int k0) {
+  if (k0 + tt::BN > s.ctx) return true;
+  // the nearest window start: a row that sees all nq drafts
+  return a.p.window > 0 && k0 < s.ctx + s.nq - a.p.window;
+}
+
+// Visibility of keys base .. base + 31 for one row.
+__device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }
+
+__device__ __forceinline__ uint32_t tree_sees(const int32_t* row, int words, int nq, int ctx, int lo, int base) {
+  uint32_t v = low_bits(ctx - base);
+  if (lo > base) v &= ~low_bits(lo - base);
+  const int j = base - ctx;                  // draft index of the first key
+  if (j > -32 && j < nq) {
+    if (j < 0) v |= tree_word(row, 0, words, nq) << -j;
+    else v |= __funnelshift_r(tree_word(row, j >> 5, words, nq), tree_word(row, (j >> 5) + 1, words, nq), j & 31);
+  }
+  return v;
+}
+
+// K-major or MN-major 128-byte-swizzled operand.  MN-major: rows of 64
+// elements along N are 128 bytes, 8-row groups along K 1024 bytes apart, the
+// two 64-element halves of N `half` bytes apart.
+__device__ __forceinline__ uint64_t sw128_desc_mn(uint32_t saddr, uint32_t half) {
+  uint64_t d = 0;
+  d |= (uint64_t)((saddr >> 4) & 0x3FFF);
+  d |= (uint64_t)((half >> 4) & 0x3FFF) << 16;
+  d |= (uint64_t)(1024 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
+
+// int8 x 4 (packed) -> two fp16x2 times scale, one rounding.
+__device__ __forceinline__ void dequant4(uint32_t x, __half2 s01, __half2 s23, uint32_t& lo, uint32_t& hi) {
+  x ^= 0x80808080u;
+  const uint32_t a = __byte_perm(x, 0x64646464u, 0x5140), b = __byte_perm(x, 0x64646464u, 0x5342);
+  const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));   // 1152
+  const __half2 p = __hmul2(__hsub2(*reinterpret_cast<const __half2*>(&a), bias), s01);
+  const __half2 q = __hmul2(__hsub2(*reinterpret_cast<const __half2*>(&b), bias), s23);
+  lo = *reinterpret_cast<const uint32_t*>(&p);
+  hi = *reinterpret_cast<const uint32_t*>(&q);
+}
+
+// Clears the halves of w whose bit in `dead` is set and those that are not
+// finite; returns 1 if a live one was not finite.
+__device__ __forceinline__ int clean2(uint32_t& w, bool dead0, bool dead1) {
+  constexpr uint32_t E = 0x7c00u;
+  int hit = 0;
+  if (dead0) w &= 0xffff0000u;
+  else if ((w & E) == E) { w &= 0xffff0000u; hit = 1; }
+  if (dead1) w &= 0x0000ffffu;
+  else if ((w & (E << 16)) == (E << 16)) { w &= 0x0000ffffu; hit = 1; }
+  return hit;
+}
+
+// Rare: a tile whose keys are checked held a value that is not finite.  The
+// converters cleared it, so that rows which do not see the key stay clean; a
+// row that sees such a key is not a number.
+static __device__ __noinline__ bool tree_poisoned(const TreeArgs& a, const TreeSeg& s, int h, const int32_t* row, int lo) {
+  const G9AttnBatch& p = a.p;
+  for (int j = s.j; j < s.j + s.n; ++j) {
+    if (!tree_checked(a, s, j * tt::BN)) continue;
+    for (int k = j * tt::BN; k < min(s.L, (j + 1) * tt::BN); ++k) {
+      if (!(tree_sees(row, a.words, s.nq, s.ctx, lo, k) & 1u)) continue;
+      const int phys = p.block_table[(int64_t)s.b * p.max_blocks + k / p.block_size];
+      if (page_bad(p, phys)) continue;
+      const int off = k % p.block_size, bs = p.block_size;
+      const uint8_t* base = p.v_cache + (int64_t)phys * p.v_page_stride + (int64_t)h * p.v_head_stride;
+      for (int d = 0; d < tt::D; ++d) {
+        __half v;
+        if (p.v_fmt == G9_VFMT_F16) {
+          v = reinterpret_cast<const __half*>(base + (int64_t)off * p.v_tok_stride)[d];
+        } else if (p.v_fmt == G9_VFMT_BF16) {
+          v = __float2half_rn(__bfloat162float(reinterpret_cast<const __nv_bfloat16*>(base + (int64_t)off * p.v_tok_stride)[d]));
+        } else {
+          const uint8_t *sc, *q;
+          if (p.v_fmt == G9_VFMT_Q8T) {
+            sc = base + 2 * ((int64_t)(d / QK) * bs + off);
+            q = base + 2 * (tt::D / QK) * bs + (int64_t)d * bs + off;
+          } else {
+            sc = base + (int64_t)off * p.v_tok_stride + d / QK * QBLOCK;
+            q = sc + 2 + d % QK;
+          }
+          v = __hmul(__short2half_rn((short)*reinterpret_cast<const int8_t*>(q)), *reinterpret_cast<const __half*>(sc));
+        }
+        if ((__half_as_ushort(v) & 0x7c00) == 0x7c00) return true;
+      }
+    }
+  }
+  return false;
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async8(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
+}
+
+// A warp's 32 raw Q8_0 token rows (136 bytes apart) -> 32 rows of an operand
+// tile [row][128] fp16 (two 64-element halves, 128-byte swizzle); lane = row.
+__device__ __forceinline__ void convert_rows(uint32_t raw, uint32_t tile, int row) {
+  const int lane = lane_id();
+  const uint32_t src = raw + lane * 136;
+  const uint32_t dst = tile + row * 128;
+  const int sw = row & 7;
+  uint32_t carry = 0;                        // the word a block shares with its neighbour
+#pragma unroll
+  for (int pair = 0; pair < 2; ++pair) {     // blocks 2*pair (starts on a word) and 2*pair + 1 (in mid-word)
+    uint32_t w[18];                          // words 17*pair .. 17*pair + 17 (pair 0), .. + 16 (pair 1)
+    if (pair == 0) {
+#pragma unroll
+      for (int i = 0; i < 9; ++i) {
+        const uint2 x = lds_u64(src + 8 * i);
+        w[2 * i] = x.x;
+        w[2 * i + 1] = x.y;
+      }
+      carry = w[17];
+    } else {
+      w[0] = carry;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint2 x = lds_u64(src + 72 + 8 * i);
+        w[2 * i + 1] = x.x;
+        w[2 * i + 2] = x.y;
+      }
+    }
+#pragma unroll
+    for (int odd = 0; odd < 2; ++odd) {
+      const uint32_t sc = odd ? w[8] >> 16 : w[0] & 0xffffu;
+      const uint32_t s2 = sc * 0x10001u;
+      const __half2 s = *reinterpret_cast<const __half2*>(&s2);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {          // 8 elements
+        uint32_t o[4];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int i = 2 * c + e;
+          const uint32_t q = odd ? w[9 + i] : __byte_perm(w[i], w[i + 1], 0x5432);
+          dequant4(q, s, s, o[2 * e], o[2 * e + 1]);
+        }
+        const int ch = (2 * pair + odd) * 4 + c;
+        sts128(dst + (ch >> 3) * (tt::TILE / 2) + (((ch & 7) ^ sw) << 4), o[0], o[1], o[2], o[3]);
+      }
+    }
+  }
+}
+
+// ===========================================================================
+template <int NQ, int VF>
+__global__ void __launch_bounds__(tt::NT, 1) tree_tc_kernel(const __grid_constant__ TreeTcParams pp) {
+  using namespace tt;
+  constexpr int E = raw_slots(NQ);
+  constexpr bool DIRECT = VF == G9_VFMT_F16 || VF == G9_VFMT_BF16;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const uint32_t sbase = smem_u32(smem);
+  const uint32_t sK = sbase, sV = sK + ST * TILE, sQ = sV + ST * TILE;
+  const uint32_t sRaw = sbase + smem_raw_off(NQ);
+  float* stat = reinterpret_cast<float*>(smem + smem_stat_off(NQ));          // [stream][m, l][row]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + smem_bar_off(NQ));
+  uint64_t *kfull = bars, *kempty = bars + 2, *vfull = bars + 4, *vempty = bars + 6, *qfull = bars + 8, *qempty = bars + 9,
+           *bs_ = bars + 10, *bp = bars + 12, *bph = bars + 14, *bo = bars + 16, *bx = bars + 18, *by = bars + 19;
+  int* misc = reinterpret_cast<int*>(bars + 20);     // 0: tensor memory, 1: abort, 2: poison, 3: total, 4: b, 5: base, 8..23: scan
+  uint32_t* tilebad = reinterpret_cast<uint32_t*>(misc + 24);                // [8], a byte per loader warp
+
+  const TreeArgs& a = pp.a;
+  const G9AttnBatch& p = a.p;
+  const int warp = warp_id(), lane = lane_id(), tid = threadIdx.x;
+  const int g = blockIdx.x / pp.Hkv, h = blockIdx.x - g * pp.Hkv;
+
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&kfull[i], 4); mbar_init(&kempty[i], 1);
+      mbar_init(&vfull[i], 4); mbar_init(&vempty[i], 1);
+      mbar_init(&bs_[i], 1); mbar_init(&bp[i], 128); mbar_init(&bph[i], 128); mbar_init(&bo[i], 1);
+    }
+    mbar_init(qfull, 64); mbar_init(qempty, 1); mbar_init(bx, 256); mbar_init(by, 256);
+    misc[1] = misc[2] = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&misc[0])));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  // ---- this CTA's range of units ----------------------------------------------
+  int total = 0;
+  for (int pass = 0; pass < 2; ++pass) {
+    const int64_t u0 = pass == 0 ? 0 : range_start(total, pp.NG, g);
+    int base = 0;
+    for (int b0 = 0; b0 < p.num_seqs; b0 += NT) {
+      const int b = b0 + tid;
+      int n = 0;
+      if (b < p.num_seqs) {
+        const TreeShape s = tree_shape<NQ>(a, b);
+        n = s.groups * s.tiles;
+      }
+      int inc = n;
+#pragma unroll
+      for (int x = 1; x < 32; x <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, inc, x);
+        if (lane >= x) inc += o;
+      }
+      __syncthreads();
+      if (lane == 31) misc[8 + warp] = inc;
+      __syncthreads();
+      int before = 0, all = 0;
+      for (int w = 0; w < NT / 32; ++w) {
+        const int x = misc[8 + w];
+        if (w < warp) before += x;
+        all += x;
+      }
+      const int first = base + before + inc - n;
+      if (pass == 1 && b < p.num_seqs) {
+        if (blockIdx.x == 0) pp.cum[b] = first;
+        if (u0 >= first && u0 < first + n) {
+          misc[4] = b;
+          misc[5] = first;
+        }
+      }
+      base += all;
+    }
+    if (pass == 0) total = base;
+  }
+  if (blockIdx.x == 0 && tid == 0) pp.cum[p.num_seqs] = total;
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = (uint32_t)misc[0];
+  TreeWalk<NQ> walk{};
+  walk.u = range_start(total, pp.NG, g);
+  walk.end = range_start(total, pp.NG, g + 1);
+  const int N = walk.end - walk.u;           // key tiles of this CTA
+  walk.b = N > 0 ? misc[4] : 0;
+  walk.base = N > 0 ? misc[5] : 0;
+  volatile int* abort_flag = &misc[1];
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REG_CTRL));
+    if (warp == 0 && lane == 0) {
+      // ======================= MMA issuer ======================================
+      constexpr uint32_t kS = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+      constexpr uint32_t kPV = kS | (VF == G9_VFMT_Q8T ? 0u : 1u << 16);
+      auto issue_s = [&](int i, int st) {
+        const uint32_t qs = sQ + (NQ == 2 ? i * TILE : 0), ks = sK + st * TILE;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t off = (kk >> 2) * (TILE / 2) + (kk & 3) * 32;
+          tc_mma_ss(tmem + i * 128, sw128_desc(qs + off), sw128_desc(ks + off), kS, kk > 0);
+        }
+        tc_commit(&bs_[i]);
+      };
+      auto issue_pv = [&](int i, int st, int half, bool first) {
+        const uint32_t vs = sV + st * TILE;
+#pragma unroll
+        for (int k4 = 0; k4 < 4; ++k4) {
+          const int kk = half * 4 + k4;
+          const uint64_t vd = VF == G9_VFMT_Q8T ? sw128_desc(vs + (kk >> 2) * (TILE / 2) + (kk & 3) * 32)
+                                                : sw128_desc_mn(vs + kk * 2048, TILE / 2);
+          tc_mma_ts(tmem + 256 + i * 128, tmem + i * 128 + kk * 8, vd, kPV, (!first || kk > 0) ? 1u : 0u);
+        }
+      };
+      bool ok = true;
+      int n0 = 0, ns = 0, cp[2] = {0, 0};    // tiles, segments and softmax steps so far
+      TreeSeg s;
+      auto pv = [&](int i, int tile, bool first) {
+        if (!mbar_wait(&bph[i], cp[i] & 1)) return false;
+        tc_fence_after();
+        issue_pv(i, tile & 1, 0, first);
+        if (!mbar_wait(&bp[i], cp[i] & 1)) return false;
+        tc_fence_after();
+        issue_pv(i, tile & 1, 1, first);
+        ++cp[i];
+        return true;
+      };
+      while (ok && walk.next(a, s)) {
+        if (!mbar_wait(qfull, ns & 1)) { ok = false; break; }
+        if constexpr (NQ == 1) {
+          for (int t = 0; ok && t < min(2, s.n); ++t) {
+            ok = mbar_wait(&kfull[(n0 + t) & 1], ((n0 + t) >> 1) & 1);
+            if (!ok) break;
+            tc_fence_after();
+            issue_s(t & 1, (n0 + t) & 1);
+            tc_commit(&kempty[(n0 + t) & 1]);
+            if (t + 1 == s.n) tc_commit(qempty);
+          }
+          for (int t = 0; ok && t < s.n; ++t) {
+            const int n = n0 + t;
+            ok = mbar_wait(&vfull[n & 1], (n >> 1) & 1) && pv(t & 1, n, t < 2);
+            if (!ok) break;
+            tc_commit(&vempty[n & 1]);
+            if (t + 2 < s.n) {
+              ok = mbar_wait(&kfull[n & 1], ((n + 2) >> 1) & 1);
+              if (!ok) break;
+              tc_fence_after();
+              issue_s(t & 1, n & 1);
+              tc_commit(&kempty[n & 1]);
+              if (t + 3 == s.n) tc_commit(qempty);
+            }
+          }
+        } else {
+          const bool two = s.rows > BM;
+          ok = mbar_wait(&kfull[n0 & 1], (n0 >> 1) & 1);
+          if (!ok) break;
+          tc_fence_after();
+          issue_s(0, n0 & 1);
+          if (two) issue_s(1, n0 & 1);
+          tc_commit(&kempty[n0 & 1]);
+          if (s.n == 1) tc_commit(qempty);
+          for (int t = 0; ok && t < s.n; ++t) {
+            const int n = n0 + t;
+            const bool more = t + 1 < s.n;
+            ok = mbar_wait(&vfull[n & 1], (n >> 1) & 1) && (!more || mbar_wait(&kfull[(n + 1) & 1], ((n + 1) >> 1) & 1));
+            ok = ok && pv(0, n, t == 0);
+            if (!ok) break;
+            if (more) issue_s(0, (n + 1) & 1);
+            if (two) {
+              ok = pv(1, n, t == 0);
+              if (!ok) break;
+              if (more) issue_s(1, (n + 1) & 1);
+            }
+            tc_commit(&vempty[n & 1]);
+            if (more) tc_commit(&kempty[(n + 1) & 1]);
+            if (t + 2 == s.n) tc_commit(qempty);
+          }
+        }
+        if (ok) {
+          tc_commit(&bo[0]);
+          tc_commit(&bo[1]);
+        }
+        n0 += s.n;
+        ++ns;
+      }
+      if (!ok) *abort_flag = 1;
+    } else if (warp >= 2) {
+      // ======================= Q rows ==========================================
+      int ns = 0;
+      TreeSeg s;
+      const int t64 = tid - 64;
+      while (walk.next(a, s)) {
+        if (ns > 0 && !mbar_wait(qempty, (ns - 1) & 1)) { *abort_flag = 1; break; }
+        for (int it = t64; it < NQ * BM * 16; it += 64) {
+          const int r = it >> 4, c = it & 15;
+          uint32_t w[4] = {0, 0, 0, 0};
+          if (r < s.rows) {
+            const int rg = s.row0 + r, t = rg / a.G;
+            const int64_t base = q_offset(p, s.b, t, h * a.G + rg - t * a.G) + 8 * c;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              w[e] = pack_half2(load_one(p.q, base + 2 * e, p.q_dtype), load_one(p.q, base + 2 * e + 1, p.q_dtype));
+          }
+          const int rr = r & (BM - 1);
+          sts128(sQ + (r >> 7) * TILE + (c >> 3) * (TILE / 2) + rr * 128 + (((c & 7) ^ (rr & 7)) << 4), w[0], w[1], w[2], w[3]);
+        }
+        fence_proxy_async();
+        mbar_arrive(qfull);
+        ++ns;
+      }
+    }
+  } else if (warp < 8) {
+    // ======================= cache rows: load and convert ========================
+    const int w = warp - 4;
+    const int bsz = p.block_size;
+    const uint32_t raw = sRaw + w * RAW;     // slot e of this warp: raw + e * 4 * RAW
+    // offsets of this lane's pieces inside 16 token rows
+    int koff[9], voff[9];
+#pragma unroll
+    for (int i = 0; i < 9; ++i) {
+      const int x = i * 32 + lane, r = x / 17;
+      koff[i] = (int)(r * p.k_tok_stride) + (x - r * 17) * 8;
+      if constexpr (VF == G9_VFMT_Q8) voff[i] = (int)(r * p.v_tok_stride) + (x - r * 17) * 8;
+      if constexpr (VF == G9_VFMT_Q8T)       // 16-byte pieces: 2 per block's scales, then one per dim
+        voff[i] = x < 8 ? 2 * (x >> 1) * bsz + 16 * (x & 1) : 2 * (D / QK) * bsz + (x - 8) * bsz;
+    }
+    TreeSeg s;
+    // a 32-key share of a tile: pages and in-page offsets of its two 16-key groups (-1: none), valid keys | checked << 8
+    struct Share { int ph0, ph1, of0, of1; uint32_t info, bad; };
+    Share nxt{-1, -1, 0, 0, 0, 0}, cur = nxt, prev = nxt;      // looked up; K loaded last; V loaded next
+    int left = 0, key0 = 0, kt = 0;          // tiles left in the segment, first key of the next tile, K tiles loaded
+    uint32_t fifo = 0;                       // infos of the V tiles loaded and not yet converted, 16 bits each
+    int nfifo = 0;
+    bool ok = true;
+    // pages of the tile after the one loaded last
+    auto lookup = [&]() {
+      if (left == 0) {
+        if (!walk.next(a, s)) return;
+        left = s.n;
+        key0 = s.j * BN;
+      }
+      const int k = key0 + 32 * w;
+      nxt.ph0 = nxt.ph1 = -1;
+      nxt.bad = 0;
+      const int32_t* bt = p.block_table + (int64_t)s.b * p.max_blocks;
+      if (k < s.L) {
+        nxt.ph0 = bt[k / bsz];
+        nxt.of0 = k % bsz;
+        if (page_bad(p, nxt.ph0)) { nxt.bad |= 1; nxt.ph0 = -1; }
+      }
+      if (k + 16 < s.L) {
+        nxt.ph1 = bt[(k + 16) / bsz];
+        nxt.of1 = (k + 16) % bsz;
+        if (page_bad(p, nxt.ph1)) { nxt.bad |= 2; nxt.ph1 = -1; }
+      }
+      if (nxt.bad && lane == 0) raise_error(ERR_BAD_PAGE);
+      nxt.info = (uint32_t)max(0, min(32, s.L - k)) | (tree_checked(a, s, key0) || nxt.bad ? 256u : 0u);
+      --left;
+      key0 += BN;
+    };
+    auto load_k = [&](uint32_t dst, int phys, int off) {
+      if (phys < 0) return;                  // stale rows: their scores are masked
+      const uint8_t* src = p.k_cache + (int64_t)phys * p.k_page_stride + (int64_t)off * p.k_tok_stride + (int64_t)h * p.k_head_stride;
+#pragma unroll
+      for (int i = 0; i < 9; ++i)
+        if (i < 8 || lane < 16) cp_async8(dst + (i * 32 + lane) * 8, src + koff[i]);
+    };
+    auto load_v = [&](uint32_t dst, int phys, int off, int grp, int vt) {
+      if constexpr (DIRECT) {
+        // straight into the operand tile; rows of a page that is not there are zeroed
+        const int c = lane & 15;
+        const uint8_t* src = p.v_cache + (int64_t)phys * p.v_page_stride + (int64_t)off * p.v_tok_stride + (int64_t)h * p.v_head_stride + 16 * c;
+        const uint32_t to = sV + (vt & 1) * TILE + (c >> 3) * (TILE / 2);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int r = 2 * i + (lane >> 4), key = 32 * w + 16 * grp + r;
+          const uint32_t at = to + key * 128 + (((c & 7) ^ (key & 7)) << 4);
+          if (phys >= 0) cp_async16(at, src + (int64_t)r * p.v_tok_stride);
+          else sts128(at, 0, 0, 0, 0);
+        }
+      } else if (phys >= 0) {
+        if constexpr (VF == G9_VFMT_Q8) {
+          const uint8_t* src = p.v_cache + (int64_t)phys * p.v_page_stride + (int64_t)off * p.v_tok_stride + (int64_t)h * p.v_head_stride;
+#pragma unroll
+          for (int i = 0; i < 9; ++i)
+            if (i < 8 || lane < 16) cp_async8(dst + grp * 2176 + (i * 32 + lane) * 8, src + voff[i]);
+        } else {
+          // the scales of 16 tokens lie 2 * off bytes, the values off bytes into their rows
+          const uint8_t* src = p.v_cache + (int64_t)phys * p.v_page_stride + (int64_t)h * p.v_head_stride + off;
+#pragma unroll
+          for (int i = 0; i < 5; ++i)
+            if (i < 4 || lane < 8) cp_async16(dst + grp * 2176 + (i * 32 + lane) * 16, src + voff[i] + (i == 0 && lane < 8 ? off : 0));
+        }
+      }
+    };
+    // item 0: K(0); odd x: K((x + 1) / 2); even x: V(x / 2 - 1)
+    auto load_item = [&](int x) {
+      const uint32_t dst = raw + (x % E) * 4 * RAW;
+      if (x == 0 || (x & 1)) {
+        prev = cur;
+        if (kt >= N) return;
+        if (x == 0) lookup();
+        cur = nxt;
+        if (lane == 0) reinterpret_cast<uint8_t*>(&tilebad[kt & 7])[w] = (uint8_t)cur.bad;
+        load_k(dst, cur.ph0, cur.of0);
+        load_k(dst + 2176, cur.ph1, cur.of1);
+        if (++kt < N) lookup();
+      } else {
+        const int vt = x / 2 - 1;
+        if constexpr (DIRECT) {
+          if (vt >= ST && !mbar_wait(&vempty[vt & 1], ((vt >> 1) - 1) & 1)) ok = false;
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) return;
+        }
+        load_v(dst, prev.ph0, prev.of0, 0, vt);
+        load_v(dst, prev.ph1, prev.of1, 1, vt);
+        fifo |= prev.info << (16 * nfifo);
+        ++nfifo;
+      }
+    };
+    auto convert_item = [&](int x) {
+      const uint32_t src = raw + (x % E) * 4 * RAW;
+      if (x == 0 || (x & 1)) {
+        const int t = (x + 1) / 2;
+        if (t >= N) return;
+        if (t >= ST && !mbar_wait(&kempty[t & 1], ((t >> 1) - 1) & 1)) ok = false;
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) return;
+        convert_rows(src, sK + (t & 1) * TILE, 32 * w + lane);
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&kfull[t & 1]);
+        return;
+      }
+      const int t = x / 2 - 1;
+      const uint32_t inf = fifo & 0xffffu;
+      fifo >>= 16;
+      --nfifo;
+      const int valid = inf & 0xff;          // keys of this warp inside the sequence
+      const bool checked = (inf & 256u) != 0;
+      const uint32_t tile = sV + (t & 1) * TILE;
+      int hit = 0;
+      if constexpr (!DIRECT) {
+        if (t >= ST && !mbar_wait(&vempty[t & 1], ((t >> 1) - 1) & 1)) ok = false;
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) return;
+      }
+      if constexpr (VF == G9_VFMT_Q8T) {
+#pragma unroll
+        for (int it = 0; it < 8; ++it) {
+          const int d = lane + 32 * (it & 3), grp = it >> 2;
+          const uint4 q = lds128(src + grp * 2176 + 128 + d * 16);
+          const uint4 s0 = lds128(src + grp * 2176 + (it & 3) * 32), s1 = lds128(src + grp * 2176 + (it & 3) * 32 + 16);
+          const uint32_t qs[4] = {q.x, q.y, q.z, q.w}, sc[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+          uint32_t o[8];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            dequant4(qs[e], *reinterpret_cast<const __half2*>(&sc[2 * e]), *reinterpret_cast<const __half2*>(&sc[2 * e + 1]),
+                     o[2 * e], o[2 * e + 1]);
+          if (checked) {
+            const int nv = valid - 16 * grp;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) hit |= clean2(o[e], 2 * e >= nv, 2 * e + 1 >= nv);
+          }
+          const int key = 32 * w + 16 * grp;
+          const uint32_t at = tile + (key >> 6) * (TILE / 2) + d * 128;
+          const int c = (key & 63) >> 3;
+          sts128(at + ((c ^ (d & 7)) << 4), o[0], o[1], o[2], o[3]);
+          sts128(at + (((c + 1) ^ (d & 7)) << 4), o[4], o[5], o[6], o[7]);
+        }
+      } else {
+        const int key = 32 * w + lane;
+        if constexpr (VF == G9_VFMT_Q8) convert_rows(src, tile, key);
+        // bf16 V becomes fp16 in place: exact for 2^-14 <= |v| < 65520, and P keeps fp16's 11 bits (in bf16 it would keep 8,
+        // which rows of few keys show)
+        if (VF == G9_VFMT_BF16 || checked) {
+          // own row: lane = key (token rows were written by this lane; 16-bit rows arrived by copies of this warp)
+          const bool dead = lane >= valid;
+          for (int c = 0; c < 16; ++c) {
+            const uint32_t at = tile + (c >> 3) * (TILE / 2) + key * 128 + (((c & 7) ^ (key & 7)) << 4);
+            uint4 x4 = lds128(at);
+            uint32_t o[4] = {x4.x, x4.y, x4.z, x4.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              if constexpr (VF == G9_VFMT_BF16)
+                o[e] = pack_half2(__uint_as_float(o[e] << 16), __uint_as_float(o[e] & 0xffff0000u));
+              if (checked) hit |= clean2(o[e], dead, dead);
+            }
+            sts128(at, o[0], o[1], o[2], o[3]);
+          }
+        }
+      }
+      if (hit) misc[2] = 1;
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&vfull[t & 1]);
+    };
+    for (int x = 0; ok && N > 0 && x < E - 1; ++x) {
+      if (x <= 2 * N) load_item(x);
+      cp_async_commit();
+    }
+    for (int x = 0; ok && N > 0 && x <= 2 * N; ++x) {
+      if (x + E - 1 <= 2 * N) load_item(x + E - 1);
+      if (!ok) break;
+      cp_async_commit();
+      cp_async_wait<E - 1>();
+      __syncwarp();
+      convert_item(x);
+      __syncwarp();
+    }
+    cp_async_wait<0>();
+    if (!ok) *abort_flag = 1;
+  } else {
+    // ======================= softmax streams =====================================
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REG_SOFT));
+    const int wi = (warp - 8) >> 2;          // stream
+    const int r = (warp & 3) * 32 + lane;    // row of the tile = TMEM lane
+    const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t tS = tmem + wi * 128 + lane_off, tO = tmem + 256 + wi * 128 + lane_off;
+    const bool general = p.softcap > 0.f || !(p.scale > 0.f);
+    int n0 = 0, ns = 0, cs = 0;              // tiles, segments, steps of this stream so far
+    bool alive = true;
+    TreeSeg s;
+    while (alive && walk.next(a, s)) {
+      const int rl = (NQ == 2 ? wi * BM : 0) + r;        // row of the group
+      const bool warp_live = (NQ == 2 ? wi * BM : 0) + (warp & 3) * 32 < s.rows;
+      const bool row_live = rl < s.rows;
+      const int rg = s.row0 + (row_live ? rl : 0), t = rg / a.G, hq = h * a.G + rg - t * a.G;
+      const int32_t* bits = tree_row(a, s.b, t);
+      const int lo = row_live ? tree_window_lo(a, bits, s.nq, s.ctx) : 0;
+      float m = -INFINITY, l = 0.f;          // log2 units
+      const bool stream_on = NQ == 1 || wi == 0 || s.rows > BM;
+      for (int j = NQ == 1 ? wi : 0; stream_on && j < s.n; j += NQ == 1 ? 2 : 1) {
+        if (!mbar_wait(&bs_[wi], cs & 1)) alive = false;
+        alive = __all_sync(0xffffffffu, alive);
+        if (!alive) break;
+        ++cs;
+        tc_fence_after();
+        if (!warp_live) {
+          mbar_arrive(&bph[wi]);
+          mbar_arrive(&bp[wi]);
+          continue;
+        }
+        const int k0 = (s.j + j) * BN;
+        const uint32_t bad = tilebad[(n0 + j) & 7];
+        const bool checked = bad || tree_checked(a, s, k0);
+        // Two passes over the scores, 64 at a time, so that a row never holds
+        // all 128 in registers: the maximum first (scores that a cap or the
+        // mask changes are written back), then the weights.
+        float mx = -INFINITY;
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          uint32_t x[2][32];
+          tmem_ld32(tS + hf * 64, x[0]);
+          tmem_ld32(tS + hf * 64 + 32, x[1]);
+          tmem_wait_ld();
+          if (general) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+              for (int e = 0; e < 32; ++e) {
+                const float y = __uint_as_float(x[c][e]);
+                x[c][e] = __float_as_uint(p.softcap > 0.f ? softcap_log2(y, a.cap_in, a.cap_out) : y * a.scale_log2);
+              }
+          }
+          if (checked) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              uint32_t v = row_live ? tree_sees(bits, a.words, s.nq, s.ctx, lo, k0 + 64 * hf + 32 * c) : 0u;
+              const uint32_t bc = bad >> (8 * (2 * hf + c));     // loader warp i holds keys 32i .. 32i + 31
+              if (bc & 1) v &= 0xffff0000u;
+              if (bc & 2) v &= 0x0000ffffu;
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if (!(v >> e & 1u)) x[c][e] = 0xff800000u;
+            }
+          }
+          if (general || checked) {
+            tmem_st32(tS + hf * 64, x[0]);
+            tmem_st32(tS + hf * 64 + 32, x[1]);
+          }
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float m0 = __uint_as_float(x[c][0]), m1 = __uint_as_float(x[c][1]);
+#pragma unroll
+            for (int e = 2; e < 30; e += 4) {
+              m0 = fmax3(m0, __uint_as_float(x[c][e]), __uint_as_float(x[c][e + 1]));
+              m1 = fmax3(m1, __uint_as_float(x[c][e + 2]), __uint_as_float(x[c][e + 3]));
+            }
+            mx = fmax3(mx, fmax3(m0, m1, __uint_as_float(x[c][30])), __uint_as_float(x[c][31]));
+          }
+        }
+        if (general || checked) tmem_wait_st();
+        if (!general) mx *= a.scale_log2;    // scale > 0: the maximum commutes with it
+        float alpha = 1.f;
+        bool rescale = false;
+        if (mx != -INFINITY && (m == -INFINITY || mx > m + kRescale)) {
+          if (m != -INFINITY) {
+            alpha = fast_exp2(m - mx);
+            l *= alpha;
+            rescale = true;
+          }
+          m = mx;
+        }
+        if (__any_sync(0xffffffffu, rescale)) {
+          // S(j) complete: every earlier PV of this stream is in O
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t o[32];
+            tmem_ld32(tO + c * 32, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            tmem_st32(tO + c * 32, o);
+          }
+        }
+        const float mu = m == -INFINITY ? 0.f : m;
+        const float sc = general ? 1.f : a.scale_log2;
+        const uint64_t sc2 = f2pack(sc, sc), nmu2 = f2pack(-mu, -mu);
+        uint64_t ls2[2] = {0ull, 0ull};
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          uint32_t x[2][32];
+          tmem_ld32(tS + hf * 64, x[0]);
+          tmem_ld32(tS + hf * 64 + 32, x[1]);
+          tmem_wait_ld();
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t pk[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const uint64_t y2 = f2fma(f2pack(__uint_as_float(x[c >> 1][(c & 1) * 16 + 2 * e]),
+                                               __uint_as_float(x[c >> 1][(c & 1) * 16 + 2 * e + 1])), sc2, nmu2);
+              float y0, y1;
+              f2unpack(y2, y0, y1);
+              y0 = fast_exp2(y0);
+              y1 = fast_exp2(y1);
+              ls2[e & 1] = f2add(ls2[e & 1], f2pack(y0, y1));
+              pk[e] = pack_half2(y0, y1);
+            }
+            // 64 weights take 32 columns: columns whose scores this row has read
+            asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+                         ::"r"(tS + hf * 32 + c * 8), "r"(pk[0]), "r"(pk[1]), "r"(pk[2]), "r"(pk[3]), "r"(pk[4]), "r"(pk[5]),
+                           "r"(pk[6]), "r"(pk[7])
+                         : "memory");
+          }
+          if (hf == 0) {                     // half of P (and any rescaled O) is in place
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(&bph[wi]);
+          }
+        }
+        float a0, a1, b0, b1;
+        f2unpack(ls2[0], a0, a1);
+        f2unpack(ls2[1], b0, b1);
+        l += (a0 + a1) + (b0 + b1);
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&bp[wi]);
+      }
+      // ---- the segment's rows ------------------------------------------------------
+      if (l != l && m == -INFINITY) m = 0.f; // only NaN scores: the row is one too
+      float w0 = 1.f, w1 = 0.f;              // weights of this stream's and the other stream's O
+      bool use0 = m != -INFINITY, use1 = false;
+      if constexpr (NQ == 1) {
+        stat[(wi * 2) * BM + r] = m;
+        stat[(wi * 2 + 1) * BM + r] = l;
+        mbar_arrive(bx);
+        if (!alive || !mbar_wait(bx, ns & 1)) alive = false;
+      }
+      if (!alive || !mbar_wait(&bo[0], ns & 1) || !mbar_wait(&bo[1], ns & 1)) alive = false;
+      alive = __all_sync(0xffffffffu, alive);
+      if (!alive) break;
+      tc_fence_after();
+      if constexpr (NQ == 1) {
+        const float m1 = stat[((wi ^ 1) * 2) * BM + r], l1 = stat[((wi ^ 1) * 2 + 1) * BM + r];
+        const float top = fmaxf(m, m1);
+        use1 = m1 != -INFINITY;
+        w0 = use0 ? fast_exp2(m - top) : 0.f;
+        w1 = use1 ? fast_exp2(m1 - top) : 0.f;
+        l = (use0 ? l * w0 : 0.f) + (use1 ? l1 * w1 : 0.f);
+        m = top;
+      }
+      if (row_live && misc[2] && tree_poisoned(a, s, h, bits, lo)) l = __int_as_float(0x7fffffff);
+      if (warp_live && stream_on) {
+        const bool whole = s.part < 0;
+        const bool any = l > 0.f || l != l;
+        float fin = 1.f;
+        if (whole) {
+          if (p.sinks && any) l += fast_exp2(sink_log2(p, hq) - m);
+          fin = (any ? 1.f / l : 0.f) * out_quant_factor(p);
+        }
+        // the streams of one row tile (NQ = 1) write half the columns each
+        const int c0 = NQ == 1 ? 2 * wi : 0, c1 = NQ == 1 ? c0 + 2 : 4;
+        const uint32_t tOther = tmem + 256 + (wi ^ 1) * 128 + lane_off;
+        const int64_t slot = ((int64_t)(2 * g + (s.part > 0 ? 1 : 0)) * pp.Hkv + h);
+        const int64_t ob = row_live ? o_offset(p, s.b, t, hq) : 0;
+#pragma unroll 1
+        for (int c = c0; c < c1; ++c) {
+          uint32_t o[32];
+          tmem_ld32(tO + c * 32, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = use0 ? __float_as_uint(__uint_as_float(o[e]) * w0) : 0u;
+          if (NQ == 1) {
+            uint32_t q[32];
+            tmem_ld32(tOther + c * 32, q);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (use1) o[e] = __float_as_uint(__uint_as_float(o[e]) + __uint_as_float(q[e]) * w1);
+          }
+          if (!row_live) continue;
+          if (!whole) {
+            float* dst = pp.po + (slot * D + c * 32) * pp.rc + rl;
+#pragma unroll
+            for (int e = 0; e < 32; ++e) dst[(int64_t)e * pp.rc] = __uint_as_float(o[e]);
+            continue;
+          }
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = any ? __float_as_uint(__uint_as_float(o[e]) * fin) : 0u;
+          if (pp.out_vec && p.out_dtype != DT_FP8) {
+            uint8_t* dst = reinterpret_cast<uint8_t*>(p.out) + (ob + c * 32) * (p.out_dtype == DT_F32 ? 4 : 2);
+            if (p.out_dtype == DT_F32) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                reinterpret_cast<uint4*>(dst)[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+            } else {
+              uint32_t y[16];
+#pragma unroll
+              for (int e = 0; e < 16; ++e)
+                y[e] = p.out_dtype == DT_F16 ? pack_half2(__uint_as_float(o[2 * e]), __uint_as_float(o[2 * e + 1]))
+                                             : pack_bf162(__uint_as_float(o[2 * e]), __uint_as_float(o[2 * e + 1]));
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                reinterpret_cast<uint4*>(dst)[e] = make_uint4(y[4 * e], y[4 * e + 1], y[4 * e + 2], y[4 * e + 3]);
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; e += 2)
+              store_out2(p.out, p.out_dtype, ob + c * 32 + e, __uint_as_float(o[e]), __uint_as_float(o[e + 1]));
+          }
+        }
+        if (!whole && row_live && (NQ == 2 || wi == 0)) {
+          pp.pml[slot * 2 * pp.rc + rl] = m;
+          pp.pml[(slot * 2 + 1) * pp.rc + rl] = l;
+        }
+      }
+      if constexpr (NQ == 1) {
+        // the other stream has read this one's O before the next segment writes it
+        tc_fence_before();
+        mbar_arrive(by);
+        if (!mbar_wait(by, ns & 1)) alive = false;
+        alive = __all_sync(0xffffffffu, alive);
+        tc_fence_after();
+      }
+      n0 += s.n;
+      ++ns;
+    }
+    if (!alive) *abort_flag = 1;
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (tid == 0 && misc[1]) raise_error(ERR_WAIT_TIMEOUT);
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Joins the partial rows of items that a range border cut: CTA (32 rows of an
+// item, kv head).  out = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s.
+// ---------------------------------------------------------------------------
+template <int NQ>
+__global__ void __launch_bounds__(256) tree_combine_kernel(const __grid_constant__ TreeTcParams pp, int row_blocks, int max_groups) {
+  using namespace tt;
+  __shared__ float rows[32][D + 1];
+  const TreeArgs& a = pp.a;
+  const G9AttnBatch& p = a.p;
+  const int rb = blockIdx.x % row_blocks;
+  const int rg = (blockIdx.x / row_blocks) % max_groups, b = blockIdx.x / row_blocks / max_groups;
+  const int h = blockIdx.y;
+  const TreeShape x = tree_shape<NQ>(a, b);
+  if (rg >= x.groups) return;
+  const int per = ((x.R + x.groups - 1) / x.groups + 31) & ~31;
+  const int nrows = max(0, min(per, x.R - rg * per));
+  if (rb * 32 >= nrows) return;
+  const int64_t T = pp.cum[p.num_seqs];
+  const int64_t u0 = (int64_t)pp.cum[b] + (int64_t)rg * x.tiles, u1 = u0 + x.tiles;
+  const int64_t ng = min((int64_t)pp.NG, T);
+  const int gf = (int)(((u0 + 1) * ng - 1) / T), gl = (int)((u1 * ng - 1) / T);
+  if (gf == gl) return;                      // written by the CTA that held all of it
+  const int lane = lane_id(), warp = warp_id();
+  const int r = rb * 32 + lane;
+  const bool live = r < nrows;
+  // the group that starts the item writes slot 2g + 1, the ones that go on 2g
+  float M = -INFINITY;
+  for (int g = gf; g <= gl; ++g) {
+    const int64_t slot = (int64_t)(2 * g + (g == gf ? 1 : 0)) * pp.Hkv + h;
+    if (live) M = fmaxf(M, pp.pml[slot * 2 * pp.rc + r]);
+  }
+  float l = 0.f, acc[16];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) acc[e] = 0.f;
+  for (int g = gf; g <= gl; ++g) {
+    const int64_t slot = (int64_t)(2 * g + (g == gf ? 1 : 0)) * pp.Hkv + h;
+    if (!live) continue;
+    const float ms = pp.pml[slot * 2 * pp.rc + r], ls = pp.pml[(slot * 2 + 1) * pp.rc + r];
+    const float w = ms == -INFINITY ? 0.f : exp2f(ms - M);
+    if (ls != ls) l = ls;                    // not a number stays so
+    if (w == 0.f) continue;
+    l += w * ls;
+    const float* src = pp.po + (slot * D + warp * 16) * pp.rc + r;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[e] += w * src[(int64_t)e * pp.rc];
+  }
+  const int row = rg * per + r, t = live ? row / a.G : 0;
+  const int hq = h * a.G + (live ? row - t * a.G : 0);
+  const bool any = l > 0.f || l != l;
+  if (p.sinks && any) l += exp2f(sink_log2(p, hq) - M);
+  const float fin = (any ? 1.f / l : 0.f) * out_quant_factor(p);
+#pragma unroll
+  for (int e = 0; e < 16; ++e) rows[lane][warp * 16 + e] = any ? acc[e] * fin : 0.f;
+  __syncthreads();
+  for (int i = warp; i < 32; i += 8) {
+    const int rr = rg * per + rb * 32 + i;
+    if (rb * 32 + i >= nrows) break;
+    const int tt_ = rr / a.G;
+    const int64_t ob = o_offset(p, b, tt_, h * a.G + rr - tt_ * a.G);
+    store_out2(p.out, p.out_dtype, ob + 2 * lane, rows[i][2 * lane], rows[i][2 * lane + 1]);
+    store_out2(p.out, p.out_dtype, ob + 64 + 2 * lane, rows[i][64 + 2 * lane], rows[i][64 + 2 * lane + 1]);
+  }
+}
+
+template <int NQ, int VF>
+cudaError_t launch_tree_tc_t(const TreeTcParams& pp, cudaStream_t stream) {
+  using namespace tt;
+  auto kern = tree_tc_kernel<NQ, VF>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(NQ));
+  if (e != cudaSuccess) return e;
+  kern<<<pp.NG * pp.Hkv, NT, smem_bytes(NQ), stream>>>(pp);
+  if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  if (pp.NG == 1) return cudaSuccess;        // nothing is cut
+  const int rows = pp.a.p.seq_q * pp.a.G, groups = (rows + NQ * BM - 1) / (NQ * BM), blocks = pp.rc / 32;
+  tree_combine_kernel<NQ><<<dim3((unsigned)(pp.a.p.num_seqs * groups * blocks), pp.Hkv), 256, 0, stream>>>(pp, blocks, groups);
+  return cudaGetLastError();
+}
+
+}  // namespace g9
