@@ -335,9 +335,12 @@ __global__ void __launch_bounds__(tt::NT, 1) tree_tc_kernel(const __grid_constan
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   // ---- this CTA's range of units ----------------------------------------------
+  // Prefix sums of the sequences' units, NT sequences at a time; the sequence
+  // that holds the range's first unit is found once the total is known, which
+  // for up to NT sequences is the same pass.
   int total = 0;
-  for (int pass = 0; pass < 2; ++pass) {
-    const int64_t u0 = pass == 0 ? 0 : range_start(total, pp.NG, g);
+  const bool one_chunk = p.num_seqs <= NT;
+  for (int pass = one_chunk ? 1 : 0; pass < 2; ++pass) {
     int base = 0;
     for (int b0 = 0; b0 < p.num_seqs; b0 += NT) {
       const int b = b0 + tid;
@@ -352,17 +355,20 @@ __global__ void __launch_bounds__(tt::NT, 1) tree_tc_kernel(const __grid_constan
         const int o = __shfl_up_sync(0xffffffffu, inc, x);
         if (lane >= x) inc += o;
       }
-      __syncthreads();
+      if (!one_chunk) __syncthreads();
       if (lane == 31) misc[8 + warp] = inc;
       __syncthreads();
       int before = 0, all = 0;
+#pragma unroll
       for (int w = 0; w < NT / 32; ++w) {
         const int x = misc[8 + w];
         if (w < warp) before += x;
         all += x;
       }
+      if (one_chunk) total = all;
       const int first = base + before + inc - n;
       if (pass == 1 && b < p.num_seqs) {
+        const int u0 = range_start(total, pp.NG, g);
         if (blockIdx.x == 0) pp.cum[b] = first;
         if (u0 >= first && u0 < first + n) {
           misc[4] = b;
@@ -371,7 +377,7 @@ __global__ void __launch_bounds__(tt::NT, 1) tree_tc_kernel(const __grid_constan
       }
       base += all;
     }
-    if (pass == 0) total = base;
+    total = base;
   }
   if (blockIdx.x == 0 && tid == 0) pp.cum[p.num_seqs] = total;
   tc_fence_before();
@@ -525,13 +531,13 @@ __global__ void __launch_bounds__(tt::NT, 1) tree_tc_kernel(const __grid_constan
     }
     TreeSeg s;
     // a 32-key share of a tile: pages and in-page offsets of its two 16-key groups (-1: none), valid keys | checked << 8
-    struct Share { int ph0, ph1, of0, of1; uint32_t info, bad; };
-    Share nxt{-1, -1, 0, 0, 0, 0}, cur = nxt, prev = nxt;      // looked up; K loaded last; V loaded next
+    struct Share { int ph0, ph1, of0, of1; uint32_t info; };
+    Share nxt{-1, -1, 0, 0, 0}, cur = nxt, prev = nxt;         // looked up; K loaded last; V loaded next
     int left = 0, key0 = 0, kt = 0;          // tiles left in the segment, first key of the next tile, K tiles loaded
     uint32_t fifo = 0;                       // infos of the V tiles loaded and not yet converted, 16 bits each
     int nfifo = 0;
     bool ok = true;
-    // pages of the tile after the one loaded last
+    // asks for the pages of the tile after the one loaded last; nothing here waits for them
     auto lookup = [&]() {
       if (left == 0) {
         if (!walk.next(a, s)) return;
@@ -539,21 +545,13 @@ __global__ void __launch_bounds__(tt::NT, 1) tree_tc_kernel(const __grid_constan
         key0 = s.j * BN;
       }
       const int k = key0 + 32 * w;
-      nxt.ph0 = nxt.ph1 = -1;
-      nxt.bad = 0;
       const int32_t* bt = p.block_table + (int64_t)s.b * p.max_blocks;
-      if (k < s.L) {
-        nxt.ph0 = bt[k / bsz];
-        nxt.of0 = k % bsz;
-        if (page_bad(p, nxt.ph0)) { nxt.bad |= 1; nxt.ph0 = -1; }
-      }
-      if (k + 16 < s.L) {
-        nxt.ph1 = bt[(k + 16) / bsz];
-        nxt.of1 = (k + 16) % bsz;
-        if (page_bad(p, nxt.ph1)) { nxt.bad |= 2; nxt.ph1 = -1; }
-      }
-      if (nxt.bad && lane == 0) raise_error(ERR_BAD_PAGE);
-      nxt.info = (uint32_t)max(0, min(32, s.L - k)) | (tree_checked(a, s, key0) || nxt.bad ? 256u : 0u);
+      const int pg0 = k / bsz, pg1 = (k + 16) / bsz;
+      nxt.ph0 = k < s.L ? bt[pg0] : -1;
+      nxt.ph1 = k + 16 < s.L ? bt[pg1] : -1;
+      nxt.of0 = k - pg0 * bsz;
+      nxt.of1 = k + 16 - pg1 * bsz;
+      nxt.info = (uint32_t)max(0, min(32, s.L - k)) | (tree_checked(a, s, key0) ? 256u : 0u);
       --left;
       key0 += BN;
     };
@@ -600,7 +598,14 @@ __global__ void __launch_bounds__(tt::NT, 1) tree_tc_kernel(const __grid_constan
         if (kt >= N) return;
         if (x == 0) lookup();
         cur = nxt;
-        if (lane == 0) reinterpret_cast<uint8_t*>(&tilebad[kt & 7])[w] = (uint8_t)cur.bad;
+        uint32_t bad = 0;                    // groups with keys on a page that is not there
+        if ((cur.info & 0xff) > 0 && page_bad(p, cur.ph0)) { bad |= 1; cur.ph0 = -1; }
+        if ((cur.info & 0xff) > 16 && page_bad(p, cur.ph1)) { bad |= 2; cur.ph1 = -1; }
+        if (bad) {
+          cur.info |= 256u;
+          if (lane == 0) raise_error(ERR_BAD_PAGE);
+        }
+        if (lane == 0) reinterpret_cast<uint8_t*>(&tilebad[kt & 7])[w] = (uint8_t)bad;
         load_k(dst, cur.ph0, cur.of0);
         load_k(dst + 2176, cur.ph1, cur.of1);
         if (++kt < N) lookup();
@@ -993,26 +998,46 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(const __grid_constant
   const int lane = lane_id(), warp = warp_id();
   const int r = rb * 32 + lane;
   const bool live = r < nrows;
-  // the group that starts the item writes slot 2g + 1, the ones that go on 2g
-  float M = -INFINITY;
-  for (int g = gf; g <= gl; ++g) {
-    const int64_t slot = (int64_t)(2 * g + (g == gf ? 1 : 0)) * pp.Hkv + h;
-    if (live) M = fmaxf(M, pp.pml[slot * 2 * pp.rc + r]);
-  }
-  float l = 0.f, acc[16];
+  // The group that starts the item writes slot 2g + 1, the ones that go on 2g.
+  // Four partials at a time: their statistics are loaded together, then their
+  // rows, so that a long item costs a few memory round trips and not one a partial.
+  constexpr int U = 4;
+  float M = -INFINITY, l = 0.f, acc[16];
 #pragma unroll
   for (int e = 0; e < 16; ++e) acc[e] = 0.f;
-  for (int g = gf; g <= gl; ++g) {
-    const int64_t slot = (int64_t)(2 * g + (g == gf ? 1 : 0)) * pp.Hkv + h;
-    if (!live) continue;
-    const float ms = pp.pml[slot * 2 * pp.rc + r], ls = pp.pml[(slot * 2 + 1) * pp.rc + r];
-    const float w = ms == -INFINITY ? 0.f : exp2f(ms - M);
-    if (ls != ls) l = ls;                    // not a number stays so
-    if (w == 0.f) continue;
-    l += w * ls;
-    const float* src = pp.po + (slot * D + warp * 16) * pp.rc + r;
+  const int rr0 = live ? r : 0;
+  for (int g0 = gf; g0 <= gl; g0 += U) {
+    float ms[U], ls[U], v[U][16];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) acc[e] += w * src[(int64_t)e * pp.rc];
+    for (int k = 0; k < U; ++k) {
+      const int g = min(g0 + k, gl);
+      const int64_t slot = (int64_t)(2 * g + (g == gf ? 1 : 0)) * pp.Hkv + h;
+      ms[k] = pp.pml[slot * 2 * pp.rc + rr0];
+      ls[k] = pp.pml[(slot * 2 + 1) * pp.rc + rr0];
+      const float* src = pp.po + (slot * D + warp * 16) * pp.rc + rr0;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) v[k][e] = src[(int64_t)e * pp.rc];
+    }
+    float top = M;
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      if (g0 + k > gl) ms[k] = -INFINITY;
+      top = fmaxf(top, ms[k]);
+    }
+    if (top == -INFINITY) continue;
+    const float shrink = M == -INFINITY ? 0.f : exp2f(M - top);
+    M = top;
+    l = shrink == 1.f ? l : l * shrink;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[e] *= shrink;
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      if (ms[k] == -INFINITY) continue;      // nothing seen: its O is zero, or was not written
+      const float w = exp2f(ms[k] - top);
+      l += w * ls[k];                        // not a number stays so
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[e] += w * v[k][e];
+    }
   }
   const int row = rg * per + r, t = live ? row / a.G : 0;
   const int hq = h * a.G + (live ? row - t * a.G : 0);
