@@ -179,7 +179,7 @@ TreePlan plan_tree(const G9AttnBatch& p) {
   const uintptr_t va = p.v_fmt == G9_VFMT_Q8 ? 8 : 16;
   if (off((uintptr_t)p.v_cache, p.v_page_stride, p.v_fmt == G9_VFMT_Q8T ? 0 : p.v_tok_stride, p.v_head_stride, va)) return pl;
   const int64_t lim = 1 << 26;               // 16 rows' offsets are held in 32 bits
-  if (std::abs(p.k_tok_stride) >= lim || std::abs(p.v_tok_stride) >= lim || p.block_size >= (1 << 20)) return pl;
+  if (std::abs(p.k_tok_stride) >= lim || std::abs(p.v_tok_stride) >= lim || p.block_size > 32768) return pl;
   const int64_t rows = (int64_t)p.seq_q * (p.num_heads_q / p.num_heads_kv);
   const int nq = rows > tt::BM ? 2 : 1;
   const int64_t groups = (rows + nq * tt::BM - 1) / (nq * tt::BM);
@@ -231,6 +231,10 @@ extern "C" cudaError_t gfx906_fa_tree_attention(const G9AttnBatch* batch, const 
   pp.Hkv = batch->num_heads_kv;
   pp.NG = pl.NG;
   pp.rc = pl.rc;
+  // Rows of odd heads start 8 bytes off a 16-byte boundary and take the 8 bytes before them along; those of even heads the 8
+  // behind them, which the next head's row holds.
+  pp.k_wide = (((uintptr_t)batch->k_cache | (uintptr_t)batch->k_page_stride | (uintptr_t)batch->k_tok_stride) & 15) == 0 &&
+              batch->k_head_stride == q8_row_bytes(tt::D) && batch->num_heads_kv % 2 == 0;
   const int64_t es = batch->out_dtype == DT_F32 ? 4 : batch->out_dtype == DT_FP8 ? 1 : 2;
   pp.out_vec = (((uintptr_t)batch->out | (uintptr_t)(batch->o_seq_stride * es) | (uintptr_t)(batch->o_tok_stride * es) |
                  (uintptr_t)(batch->o_head_stride * es)) & 15) == 0;

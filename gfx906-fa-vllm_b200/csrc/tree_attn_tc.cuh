@@ -16,13 +16,15 @@
 // the same number of tiles whatever the lengths.  An item cut by a range border
 // leaves partial rows that tree_combine_kernel joins.
 //
-// CTA, 512 threads:
-//   warp 0       issues every tcgen05.mma from one thread
-//   warps 2-3    bring the row tile(s) of Q into shared memory (fp16)
-//   warps 4-7    load cache rows (cp.async, raw) and convert: K to [key][d], V to
-//                [d][key] (page-transposed Q8_0) or [key][d] (token rows); a warp owns 32 keys of
-//                a tile, so loading and converting need no barrier between warps
-//   warps 8-15   two softmax streams, a thread a row (row = TMEM lane)
+// CTA, 12 warps of 168 registers (16 warps hold 128 each, where the loaders and
+// the softmax spill, and L1 is too small beside 227 KB of shared memory for
+// what they spill):
+//   warps 0-7    two softmax streams, a thread a row (row = TMEM lane).  A stream's first thread
+//                also issues its tcgen05.mma: the stream has nothing else to do until its next
+//                scores are there, so no warp is spent on it.
+//   warps 8-11   load cache rows and convert: K to [key][d], V to [d][key] (page-transposed Q8_0)
+//                or [key][d] (token rows); a warp owns 32 keys of a tile, so loading and converting
+//                need no barrier between warps
 // One query tile (NQ = 1): the streams take alternate key tiles of the same
 // rows, each with its own running maximum, sum and accumulator, so that one
 // stream's softmax runs under the other's MMAs; they are joined through TMEM at
@@ -43,20 +45,17 @@ constexpr int BM = 128;
 constexpr int BN = 128;
 constexpr int ST = 2;                        // K and V stages
 constexpr int TILE = BM * D * 2;             // 32 KB
-constexpr int NT = 512;
-constexpr int RAW = 32 * (D / QK) * QBLOCK;  // a warp's 32 raw rows: 4352 bytes
-// launch 512 x 128 registers = 128*REG_CTRL + 128*REG_LOAD + 256*REG_SOFT
-constexpr int REG_CTRL = 56;
-constexpr int REG_LOAD = 128;                // as launched
-constexpr int REG_SOFT = 160;
-static_assert(128 * REG_CTRL + 128 * REG_LOAD + 256 * REG_SOFT <= NT * 128, "register split exceeds the launch budget");
+constexpr int NT = 384;
+constexpr int PITCH = 144;                   // raw Q8_0 rows: 136 bytes, up to 8 before or behind them
+constexpr int RAW = 16 * PITCH;              // a warp's slot: 16 raw rows
 constexpr float kRescale = 8.0f;             // log2 units
 
-// raw slots a warp rotates through, in shared memory left over by the tiles
-constexpr int raw_slots(int nq) { return nq == 1 ? 3 : 2; }
+// raw slots a warp rotates through, in the shared memory that the tiles leave
+constexpr int raw_slots(int nq) { return nq == 1 ? 7 : 3; }
 constexpr int smem_raw_off(int nq) { return (2 * ST + nq) * TILE; }
 constexpr int smem_stat_off(int nq) { return smem_raw_off(nq) + raw_slots(nq) * 4 * RAW; }
-constexpr int smem_bar_off(int nq) { return smem_stat_off(nq) + (nq == 1 ? 2 * 2 * BM * 4 : 0); }
+constexpr int smem_share_off(int nq) { return smem_stat_off(nq) + (nq == 1 ? 2 * 2 * BM * 4 : 0); }
+constexpr int smem_bar_off(int nq) { return smem_share_off(nq) + 4 * 8 * 16 + 4 * 256; }
 constexpr int smem_bytes(int nq) { return smem_bar_off(nq) + 512; }
 static_assert(smem_bytes(1) <= 232448 && smem_bytes(2) <= 232448, "shared memory");
 }  // namespace tt
@@ -65,6 +64,7 @@ struct TreeTcParams {
   TreeArgs a;
   int Hkv, NG;
   int rc;                        // rows of a partial block (a multiple of 32)
+  int k_wide;                    // K rows may be copied as 16-byte pieces (even head counts)
   int out_vec;                   // output rows may be written 16 bytes at a time
   int* cum;                      // [num_seqs + 1] first unit of each sequence
   float* po;                     // [2 * NG][Hkv][128][rc] partial O
@@ -240,61 +240,51 @@ __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commi
 template <int N>
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-__device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
-}
-__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+// arrives on `bar` when this thread's copies so far have landed
+__device__ __forceinline__ void cp_async_mbar_arrive(uint64_t* bar) { cp_async_arrive_noinc(bar); }
+
+// a load that stays where it is written, ahead of the work that hides it
+__device__ __forceinline__ uint4 ldg16_early(const void* p) {
   uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
   return v;
 }
 
-// A warp's 32 raw Q8_0 token rows (136 bytes apart) -> 32 rows of an operand
-// tile [row][128] fp16 (two 64-element halves, 128-byte swizzle); lane = row.
-__device__ __forceinline__ void convert_rows(uint32_t raw, uint32_t tile, int row) {
-  const int lane = lane_id();
-  const uint32_t src = raw + lane * 136;
-  const uint32_t dst = tile + row * 128;
+__device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+// 16 raw Q8_0 token rows (PITCH bytes apart, starting 8 * ODD bytes into them)
+// -> rows row0 .. row0 + 15 of an operand tile [row][128] fp16 (two 64-element
+// halves, 128-byte swizzle).  Lane (row, f) converts blocks 2f and 2f + 1: the
+// 68 bytes from 68 f on, read as five aligned 16-byte words.
+template <int ODD>
+__device__ __forceinline__ void convert_rows(const uint8_t* raw, uint8_t* tile, int row0) {
+  const int lane = lane_id(), f = lane & 1, row = row0 + (lane >> 1);
+  const uint4* src = reinterpret_cast<const uint4*>(raw + (lane >> 1) * tt::PITCH + 64 * f);
+  uint32_t w[20];
+#pragma unroll
+  for (int i = 0; i < 5; ++i) {
+    const uint4 x = src[i];
+    w[4 * i] = x.x; w[4 * i + 1] = x.y; w[4 * i + 2] = x.z; w[4 * i + 3] = x.w;
+  }
+  uint32_t y[17];                            // the 68 bytes: they start a word later for f = 1
+#pragma unroll
+  for (int i = 0; i < 17; ++i) y[i] = f ? w[i + 2 * ODD + 1] : w[i + 2 * ODD];
+  const uint32_t s0 = (y[0] & 0xffffu) * 0x10001u, s1 = (y[8] >> 16) * 0x10001u;
+  uint8_t* dst = tile + f * (tt::TILE / 2) + row * 128;
   const int sw = row & 7;
-  uint32_t carry = 0;                        // the word a block shares with its neighbour
 #pragma unroll
-  for (int pair = 0; pair < 2; ++pair) {     // blocks 2*pair (starts on a word) and 2*pair + 1 (in mid-word)
-    uint32_t w[18];                          // words 17*pair .. 17*pair + 17 (pair 0), .. + 16 (pair 1)
-    if (pair == 0) {
+  for (int c = 0; c < 8; ++c) {              // 8 elements
+    uint32_t o[4];
 #pragma unroll
-      for (int i = 0; i < 9; ++i) {
-        const uint2 x = lds_u64(src + 8 * i);
-        w[2 * i] = x.x;
-        w[2 * i + 1] = x.y;
-      }
-      carry = w[17];
-    } else {
-      w[0] = carry;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint2 x = lds_u64(src + 72 + 8 * i);
-        w[2 * i + 1] = x.x;
-        w[2 * i + 2] = x.y;
-      }
+    for (int e = 0; e < 2; ++e) {
+      const int i = 2 * (c & 3) + e;
+      // the first block's values start in mid-word, the second's on a word
+      const uint32_t q = c < 4 ? __byte_perm(y[i], y[i + 1], 0x5432) : y[9 + i];
+      const __half2 s = *reinterpret_cast<const __half2*>(c < 4 ? &s0 : &s1);
+      dequant4(q, s, s, o[2 * e], o[2 * e + 1]);
     }
-#pragma unroll
-    for (int odd = 0; odd < 2; ++odd) {
-      const uint32_t sc = odd ? w[8] >> 16 : w[0] & 0xffffu;
-      const uint32_t s2 = sc * 0x10001u;
-      const __half2 s = *reinterpret_cast<const __half2*>(&s2);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {          // 8 elements
-        uint32_t o[4];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int i = 2 * c + e;
-          const uint32_t q = odd ? w[9 + i] : __byte_perm(w[i], w[i + 1], 0x5432);
-          dequant4(q, s, s, o[2 * e], o[2 * e + 1]);
-        }
-        const int ch = (2 * pair + odd) * 4 + c;
-        sts128(dst + (ch >> 3) * (tt::TILE / 2) + (((ch & 7) ^ sw) << 4), o[0], o[1], o[2], o[3]);
-      }
-    }
+    *reinterpret_cast<uint4*>(dst + ((c ^ sw) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
   }
 }
 
@@ -307,12 +297,11 @@ __global__ void __launch_bounds__(tt::NT, 1) tree_tc_kernel(const __grid_constan
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t sbase = smem_u32(smem);
   const uint32_t sK = sbase, sV = sK + ST * TILE, sQ = sV + ST * TILE;
-  const uint32_t sRaw = sbase + smem_raw_off(NQ);
   float* stat = reinterpret_cast<float*>(smem + smem_stat_off(NQ));          // [stream][m, l][row]
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + smem_bar_off(NQ));
-  uint64_t *kfull = bars, *kempty = bars + 2, *vfull = bars + 4, *vempty = bars + 6, *qfull = bars + 8, *qempty = bars + 9,
-           *bs_ = bars + 10, *bp = bars + 12, *bph = bars + 14, *bo = bars + 16, *bx = bars + 18, *by = bars + 19;
-  int* misc = reinterpret_cast<int*>(bars + 20);     // 0: tensor memory, 1: abort, 2: poison, 3: total, 4: b, 5: base, 8..23: scan
+  uint64_t *kfull = bars, *kempty = bars + 2, *vfull = bars + 4, *vempty = bars + 6, *qfull = bars + 8, *bs_ = bars + 10,
+           *bp = bars + 12, *bo = bars + 14, *bx = bars + 16, *by = bars + 17, *vraw = bars + 18;
+  int* misc = reinterpret_cast<int*>(bars + 24);     // 0: tensor memory, 1: abort, 2: poison, 3: total, 4: b, 5: base, 8..23: scan
   uint32_t* tilebad = reinterpret_cast<uint32_t*>(misc + 24);                // [8], a byte per loader warp
 
   const TreeArgs& a = pp.a;
@@ -322,15 +311,18 @@ __global__ void __launch_bounds__(tt::NT, 1) tree_tc_kernel(const __grid_constan
 
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&kfull[i], 4); mbar_init(&kempty[i], 1);
-      mbar_init(&vfull[i], 4); mbar_init(&vempty[i], 1);
-      mbar_init(&bs_[i], 1); mbar_init(&bp[i], 128); mbar_init(&bph[i], 128); mbar_init(&bo[i], 1);
+      // a tile is free when every stream that reads it is done: one (NQ = 1) or both
+      mbar_init(&kfull[i], 4); mbar_init(&kempty[i], NQ);
+      mbar_init(&vfull[i], 4); mbar_init(&vempty[i], NQ);
+      mbar_init(&bs_[i], 1); mbar_init(&bp[i], 128); mbar_init(&bo[i], 1);
+      mbar_init(&qfull[i], NQ == 1 ? 256 : 128);
     }
-    mbar_init(qfull, 64); mbar_init(qempty, 1); mbar_init(bx, 256); mbar_init(by, 256);
+    for (int i = 0; i < 4; ++i) mbar_init(&vraw[i], 32);
+    mbar_init(bx, 256); mbar_init(by, 256);
     misc[1] = misc[2] = 0;
     fence_barrier_init();
   }
-  if (warp == 1) {
+  if (warp == 8) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&misc[0])));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
@@ -392,153 +384,33 @@ __global__ void __launch_bounds__(tt::NT, 1) tree_tc_kernel(const __grid_constan
   walk.base = N > 0 ? misc[5] : 0;
   volatile int* abort_flag = &misc[1];
 
-  if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REG_CTRL));
-    if (warp == 0 && lane == 0) {
-      // ======================= MMA issuer ======================================
-      constexpr uint32_t kS = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
-      constexpr uint32_t kPV = kS | (VF == G9_VFMT_Q8T ? 0u : 1u << 16);
-      auto issue_s = [&](int i, int st) {
-        const uint32_t qs = sQ + (NQ == 2 ? i * TILE : 0), ks = sK + st * TILE;
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t off = (kk >> 2) * (TILE / 2) + (kk & 3) * 32;
-          tc_mma_ss(tmem + i * 128, sw128_desc(qs + off), sw128_desc(ks + off), kS, kk > 0);
-        }
-        tc_commit(&bs_[i]);
-      };
-      auto issue_pv = [&](int i, int st, int half, bool first) {
-        const uint32_t vs = sV + st * TILE;
-#pragma unroll
-        for (int k4 = 0; k4 < 4; ++k4) {
-          const int kk = half * 4 + k4;
-          const uint64_t vd = VF == G9_VFMT_Q8T ? sw128_desc(vs + (kk >> 2) * (TILE / 2) + (kk & 3) * 32)
-                                                : sw128_desc_mn(vs + kk * 2048, TILE / 2);
-          tc_mma_ts(tmem + 256 + i * 128, tmem + i * 128 + kk * 8, vd, kPV, (!first || kk > 0) ? 1u : 0u);
-        }
-      };
-      bool ok = true;
-      int n0 = 0, ns = 0, cp[2] = {0, 0};    // tiles, segments and softmax steps so far
-      TreeSeg s;
-      auto pv = [&](int i, int tile, bool first) {
-        if (!mbar_wait(&bph[i], cp[i] & 1)) return false;
-        tc_fence_after();
-        issue_pv(i, tile & 1, 0, first);
-        if (!mbar_wait(&bp[i], cp[i] & 1)) return false;
-        tc_fence_after();
-        issue_pv(i, tile & 1, 1, first);
-        ++cp[i];
-        return true;
-      };
-      while (ok && walk.next(a, s)) {
-        if (!mbar_wait(qfull, ns & 1)) { ok = false; break; }
-        if constexpr (NQ == 1) {
-          for (int t = 0; ok && t < min(2, s.n); ++t) {
-            ok = mbar_wait(&kfull[(n0 + t) & 1], ((n0 + t) >> 1) & 1);
-            if (!ok) break;
-            tc_fence_after();
-            issue_s(t & 1, (n0 + t) & 1);
-            tc_commit(&kempty[(n0 + t) & 1]);
-            if (t + 1 == s.n) tc_commit(qempty);
-          }
-          for (int t = 0; ok && t < s.n; ++t) {
-            const int n = n0 + t;
-            ok = mbar_wait(&vfull[n & 1], (n >> 1) & 1) && pv(t & 1, n, t < 2);
-            if (!ok) break;
-            tc_commit(&vempty[n & 1]);
-            if (t + 2 < s.n) {
-              ok = mbar_wait(&kfull[n & 1], ((n + 2) >> 1) & 1);
-              if (!ok) break;
-              tc_fence_after();
-              issue_s(t & 1, n & 1);
-              tc_commit(&kempty[n & 1]);
-              if (t + 3 == s.n) tc_commit(qempty);
-            }
-          }
-        } else {
-          const bool two = s.rows > BM;
-          ok = mbar_wait(&kfull[n0 & 1], (n0 >> 1) & 1);
-          if (!ok) break;
-          tc_fence_after();
-          issue_s(0, n0 & 1);
-          if (two) issue_s(1, n0 & 1);
-          tc_commit(&kempty[n0 & 1]);
-          if (s.n == 1) tc_commit(qempty);
-          for (int t = 0; ok && t < s.n; ++t) {
-            const int n = n0 + t;
-            const bool more = t + 1 < s.n;
-            ok = mbar_wait(&vfull[n & 1], (n >> 1) & 1) && (!more || mbar_wait(&kfull[(n + 1) & 1], ((n + 1) >> 1) & 1));
-            ok = ok && pv(0, n, t == 0);
-            if (!ok) break;
-            if (more) issue_s(0, (n + 1) & 1);
-            if (two) {
-              ok = pv(1, n, t == 0);
-              if (!ok) break;
-              if (more) issue_s(1, (n + 1) & 1);
-            }
-            tc_commit(&vempty[n & 1]);
-            if (more) tc_commit(&kempty[(n + 1) & 1]);
-            if (t + 2 == s.n) tc_commit(qempty);
-          }
-        }
-        if (ok) {
-          tc_commit(&bo[0]);
-          tc_commit(&bo[1]);
-        }
-        n0 += s.n;
-        ++ns;
-      }
-      if (!ok) *abort_flag = 1;
-    } else if (warp >= 2) {
-      // ======================= Q rows ==========================================
-      int ns = 0;
-      TreeSeg s;
-      const int t64 = tid - 64;
-      while (walk.next(a, s)) {
-        if (ns > 0 && !mbar_wait(qempty, (ns - 1) & 1)) { *abort_flag = 1; break; }
-        for (int it = t64; it < NQ * BM * 16; it += 64) {
-          const int r = it >> 4, c = it & 15;
-          uint32_t w[4] = {0, 0, 0, 0};
-          if (r < s.rows) {
-            const int rg = s.row0 + r, t = rg / a.G;
-            const int64_t base = q_offset(p, s.b, t, h * a.G + rg - t * a.G) + 8 * c;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              w[e] = pack_half2(load_one(p.q, base + 2 * e, p.q_dtype), load_one(p.q, base + 2 * e + 1, p.q_dtype));
-          }
-          const int rr = r & (BM - 1);
-          sts128(sQ + (r >> 7) * TILE + (c >> 3) * (TILE / 2) + rr * 128 + (((c & 7) ^ (rr & 7)) << 4), w[0], w[1], w[2], w[3]);
-        }
-        fence_proxy_async();
-        mbar_arrive(qfull);
-        ++ns;
-      }
-    }
-  } else if (warp < 8) {
+  if (warp >= 8) {
     // ======================= cache rows: load and convert ========================
-    const int w = warp - 4;
+    const int w = warp - 8;
     const int bsz = p.block_size;
-    const uint32_t raw = sRaw + w * RAW;     // slot e of this warp: raw + e * 4 * RAW
-    // offsets of this lane's pieces inside 16 token rows
-    int koff[9], voff[9];
+    uint8_t* raw = smem + smem_raw_off(NQ) + w * E * RAW;      // this warp's slots
+    // pages of the last 8 tiles looked up: (page, offset) of the two 16-key groups, keys inside the sequence | checked << 8
+    int4* shares = reinterpret_cast<int4*>(smem + smem_share_off(NQ)) + 8 * w;
+    uint32_t* vscale = reinterpret_cast<uint32_t*>(smem + smem_share_off(NQ) + 4 * 8 * 16 + w * 256);
+    const int odd = pp.k_wide && (h & 1);    // the row starts 8 bytes into its first 16-byte piece
+    const uint8_t* kbase = p.k_cache + (int64_t)h * p.k_head_stride - 8 * odd;
+    const uint8_t* vbase = p.v_cache + (int64_t)h * p.v_head_stride;
+    // offsets of this lane's pieces of 16 token rows: 9 pieces of 16 bytes a row, or 17 of 8
+    int koff[5], kdst[5];
 #pragma unroll
-    for (int i = 0; i < 9; ++i) {
-      const int x = i * 32 + lane, r = x / 17;
-      koff[i] = (int)(r * p.k_tok_stride) + (x - r * 17) * 8;
-      if constexpr (VF == G9_VFMT_Q8) voff[i] = (int)(r * p.v_tok_stride) + (x - r * 17) * 8;
-      if constexpr (VF == G9_VFMT_Q8T)       // 16-byte pieces: 2 per block's scales, then one per dim
-        voff[i] = x < 8 ? 2 * (x >> 1) * bsz + 16 * (x & 1) : 2 * (D / QK) * bsz + (x - 8) * bsz;
+    for (int i = 0; i < 5; ++i) {
+      const int x = i * 32 + lane, r = x / 9;
+      koff[i] = (int)(r * p.k_tok_stride) + (x - r * 9) * 16;
+      kdst[i] = r * PITCH + (x - r * 9) * 16;
     }
     TreeSeg s;
-    // a 32-key share of a tile: pages and in-page offsets of its two 16-key groups (-1: none), valid keys | checked << 8
-    struct Share { int ph0, ph1, of0, of1; uint32_t info; };
-    Share nxt{-1, -1, 0, 0, 0}, cur = nxt, prev = nxt;         // looked up; K loaded last; V loaded next
-    int left = 0, key0 = 0, kt = 0;          // tiles left in the segment, first key of the next tile, K tiles loaded
-    uint32_t fifo = 0;                       // infos of the V tiles loaded and not yet converted, 16 bits each
-    int nfifo = 0;
+    int left = 0, key0 = 0;                  // tiles left in the segment, first key of the next tile
+    int looked = 0;                          // tiles looked up
+    int ph0 = -1, ph1 = -1, of0 = 0, of1 = 0, info = 0;        // the last of them
     bool ok = true;
-    // asks for the pages of the tile after the one loaded last; nothing here waits for them
+    // asks for the next tile's pages; nothing here waits for them
     auto lookup = [&]() {
+      if (looked >= N) return;
       if (left == 0) {
         if (!walk.next(a, s)) return;
         left = s.n;
@@ -547,142 +419,227 @@ __global__ void __launch_bounds__(tt::NT, 1) tree_tc_kernel(const __grid_constan
       const int k = key0 + 32 * w;
       const int32_t* bt = p.block_table + (int64_t)s.b * p.max_blocks;
       const int pg0 = k / bsz, pg1 = (k + 16) / bsz;
-      nxt.ph0 = k < s.L ? bt[pg0] : -1;
-      nxt.ph1 = k + 16 < s.L ? bt[pg1] : -1;
-      nxt.of0 = k - pg0 * bsz;
-      nxt.of1 = k + 16 - pg1 * bsz;
-      nxt.info = (uint32_t)max(0, min(32, s.L - k)) | (tree_checked(a, s, key0) ? 256u : 0u);
+      ph0 = k < s.L ? bt[pg0] : -1;
+      ph1 = k + 16 < s.L ? bt[pg1] : -1;
+      of0 = k - pg0 * bsz;
+      of1 = k + 16 - pg1 * bsz;
+      info = max(0, min(32, s.L - k)) | (tree_checked(a, s, key0) ? 256 : 0);
       --left;
       key0 += BN;
+      ++looked;
     };
-    auto load_k = [&](uint32_t dst, int phys, int off) {
-      if (phys < 0) return;                  // stale rows: their scores are masked
-      const uint8_t* src = p.k_cache + (int64_t)phys * p.k_page_stride + (int64_t)off * p.k_tok_stride + (int64_t)h * p.k_head_stride;
-#pragma unroll
-      for (int i = 0; i < 9; ++i)
-        if (i < 8 || lane < 16) cp_async8(dst + (i * 32 + lane) * 8, src + koff[i]);
+    // notes what the last lookup brought
+    auto settle = [&]() {
+      uint32_t bad = 0;                      // groups with keys on a page that is not there
+      if ((info & 0xff) > 0 && page_bad(p, ph0)) { bad |= 1; ph0 = -1; }
+      if ((info & 0xff) > 16 && page_bad(p, ph1)) { bad |= 2; ph1 = -1; }
+      if (bad) {
+        info |= 256;
+        if (lane == 0) raise_error(ERR_BAD_PAGE);
+      }
+      const int t = looked - 1;
+      if (lane == 0) {
+        reinterpret_cast<uint8_t*>(&tilebad[t & 7])[w] = (uint8_t)bad;
+        shares[t & 7] = make_int4(ph0, ph1, of0 | of1 << 16, info);
+      }
+      __syncwarp();
     };
-    auto load_v = [&](uint32_t dst, int phys, int off, int grp, int vt) {
-      if constexpr (DIRECT) {
-        // straight into the operand tile; rows of a page that is not there are zeroed
-        const int c = lane & 15;
-        const uint8_t* src = p.v_cache + (int64_t)phys * p.v_page_stride + (int64_t)off * p.v_tok_stride + (int64_t)h * p.v_head_stride + 16 * c;
-        const uint32_t to = sV + (vt & 1) * TILE + (c >> 3) * (TILE / 2);
+    // 16 token rows of 136 bytes into a raw slot; stale rows of a page that is not there are masked or cleared later
+    auto load_rows = [&](uint32_t dst, const uint8_t* src, int64_t tok_stride, bool wide) {
+      if (wide) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int r = 2 * i + (lane >> 4), key = 32 * w + 16 * grp + r;
-          const uint32_t at = to + key * 128 + (((c & 7) ^ (key & 7)) << 4);
-          if (phys >= 0) cp_async16(at, src + (int64_t)r * p.v_tok_stride);
-          else sts128(at, 0, 0, 0, 0);
+        for (int i = 0; i < 5; ++i)
+          if (i < 4 || lane < 16) cp_async16(dst + kdst[i], src + koff[i]);
+      } else {
+#pragma unroll 3
+        for (int x = lane; x < 272; x += 32) {
+          const int r = x / 17, c = x - r * 17;
+          cp_async8(dst + r * PITCH + c * 8, src + r * tok_stride + c * 8);
         }
-      } else if (phys >= 0) {
-        if constexpr (VF == G9_VFMT_Q8) {
-          const uint8_t* src = p.v_cache + (int64_t)phys * p.v_page_stride + (int64_t)off * p.v_tok_stride + (int64_t)h * p.v_head_stride;
-#pragma unroll
-          for (int i = 0; i < 9; ++i)
-            if (i < 8 || lane < 16) cp_async8(dst + grp * 2176 + (i * 32 + lane) * 8, src + voff[i]);
+      }
+    };
+    // The raw queue holds 16-row groups in the order they are converted: K of
+    // tile 0, then K of tile n + 1 and (token-row V) V of tile n.
+    constexpr int PER = VF == G9_VFMT_Q8 ? 4 : 2;              // groups a tile
+    const int groups = PER * N;
+    int issued = 0, taken = 0;
+    auto issue = [&]() {
+      if (issued < groups) {
+        // which tile, which operand
+        int t, isv = 0, grp;
+        if (PER == 2) {
+          t = issued >> 1;
+          grp = issued & 1;
+        } else if (issued < 2) {
+          t = 0;
+          grp = issued;
         } else {
-          // the scales of 16 tokens lie 2 * off bytes, the values off bytes into their rows
-          const uint8_t* src = p.v_cache + (int64_t)phys * p.v_page_stride + (int64_t)h * p.v_head_stride + off;
-#pragma unroll
-          for (int i = 0; i < 5; ++i)
-            if (i < 4 || lane < 8) cp_async16(dst + grp * 2176 + (i * 32 + lane) * 16, src + voff[i] + (i == 0 && lane < 8 ? off : 0));
+          const int y = issued - 2, n = y >> 2;                // K(n + 1) two groups, V(n) two groups; the last tile has V only
+          const bool last = n == N - 1;
+          grp = y & 1;
+          isv = last || (y & 2);
+          t = isv ? n : n + 1;
         }
+        if (!isv && grp == 0) {              // a new tile: its pages were asked for a tile ago
+          settle();
+          lookup();
+        }
+        const int4 sh = shares[t & 7];
+        const int phys = grp ? sh.y : sh.x, off = grp ? sh.z >> 16 : sh.z & 0xffff;
+        if (phys >= 0) {
+          const uint32_t dst = smem_u32(raw + (issued % E) * RAW);
+          if (!isv) load_rows(dst, kbase + (int64_t)phys * p.k_page_stride + (int64_t)off * p.k_tok_stride, p.k_tok_stride, pp.k_wide);
+          else load_rows(dst, vbase + (int64_t)phys * p.v_page_stride + (int64_t)off * p.v_tok_stride, p.v_tok_stride, false);
+        }
+        ++issued;
       }
+      cp_async_commit();
     };
-    // item 0: K(0); odd x: K((x + 1) / 2); even x: V(x / 2 - 1)
-    auto load_item = [&](int x) {
-      const uint32_t dst = raw + (x % E) * 4 * RAW;
-      if (x == 0 || (x & 1)) {
-        prev = cur;
-        if (kt >= N) return;
-        if (x == 0) lookup();
-        cur = nxt;
-        uint32_t bad = 0;                    // groups with keys on a page that is not there
-        if ((cur.info & 0xff) > 0 && page_bad(p, cur.ph0)) { bad |= 1; cur.ph0 = -1; }
-        if ((cur.info & 0xff) > 16 && page_bad(p, cur.ph1)) { bad |= 2; cur.ph1 = -1; }
-        if (bad) {
-          cur.info |= 256u;
-          if (lane == 0) raise_error(ERR_BAD_PAGE);
-        }
-        if (lane == 0) reinterpret_cast<uint8_t*>(&tilebad[kt & 7])[w] = (uint8_t)bad;
-        load_k(dst, cur.ph0, cur.of0);
-        load_k(dst + 2176, cur.ph1, cur.of1);
-        if (++kt < N) lookup();
-      } else {
-        const int vt = x / 2 - 1;
-        if constexpr (DIRECT) {
-          if (vt >= ST && !mbar_wait(&vempty[vt & 1], ((vt >> 1) - 1) & 1)) ok = false;
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) return;
-        }
-        load_v(dst, prev.ph0, prev.of0, 0, vt);
-        load_v(dst, prev.ph1, prev.of1, 1, vt);
-        fifo |= prev.info << (16 * nfifo);
-        ++nfifo;
-      }
+    // the oldest group has arrived
+    auto take = [&]() -> const uint8_t* {
+      cp_async_wait<E - 2>();
+      __syncwarp();
+      return raw + (taken % E) * RAW;
     };
-    auto convert_item = [&](int x) {
-      const uint32_t src = raw + (x % E) * 4 * RAW;
-      if (x == 0 || (x & 1)) {
-        const int t = (x + 1) / 2;
-        if (t >= N) return;
-        if (t >= ST && !mbar_wait(&kempty[t & 1], ((t >> 1) - 1) & 1)) ok = false;
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) return;
-        convert_rows(src, sK + (t & 1) * TILE, 32 * w + lane);
-        fence_proxy_async();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&kfull[t & 1]);
-        return;
+    auto release = [&]() {
+      __syncwarp();                          // every lane has read the slot
+      ++taken;
+      issue();
+    };
+    auto convert_k = [&](int t) {
+      if (t >= ST && !mbar_wait(&kempty[t & 1], ((t >> 1) - 1) & 1)) ok = false;
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) return;
+      uint8_t* tile = smem + (t & 1) * TILE;
+#pragma unroll 1
+      for (int grp = 0; grp < 2; ++grp) {
+        const uint8_t* src = take();
+        if (odd) convert_rows<1>(src, tile, 32 * w + 16 * grp);
+        else convert_rows<0>(src, tile, 32 * w + 16 * grp);
+        release();
       }
-      const int t = x / 2 - 1;
-      const uint32_t inf = fifo & 0xffffu;
-      fifo >>= 16;
-      --nfifo;
-      const int valid = inf & 0xff;          // keys of this warp inside the sequence
-      const bool checked = (inf & 256u) != 0;
-      const uint32_t tile = sV + (t & 1) * TILE;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&kfull[t & 1]);
+    };
+    auto wait_vempty = [&](int t) {
+      if (t >= ST && !mbar_wait(&vempty[t & 1], ((t >> 1) - 1) & 1)) ok = false;
+      ok = __all_sync(0xffffffffu, ok);
+    };
+    if (N > 0) {
+      lookup();
+#pragma unroll 1
+      for (int i = 0; i < E - 1; ++i) issue();
+      convert_k(0);
+    }
+#pragma unroll 1
+    for (int t = 0; ok && t < N; ++t) {
+      const int4 sh = shares[t & 7];
+      const int valid = sh.w & 0xff;         // keys of this warp inside the sequence
+      const bool checked = (sh.w & 256) != 0;
+      uint8_t* tile = smem + (ST + (t & 1)) * TILE;
       int hit = 0;
-      if constexpr (!DIRECT) {
-        if (t >= ST && !mbar_wait(&vempty[t & 1], ((t >> 1) - 1) & 1)) ok = false;
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) return;
-      }
       if constexpr (VF == G9_VFMT_Q8T) {
+        // Page-transposed records go through registers: a lane's 16 bytes are 16
+        // keys of one dim.  They are asked for before the next K tile is converted.
+        uint4 q[2][4];
+        uint32_t sc[2];
 #pragma unroll
-        for (int it = 0; it < 8; ++it) {
-          const int d = lane + 32 * (it & 3), grp = it >> 2;
-          const uint4 q = lds128(src + grp * 2176 + 128 + d * 16);
-          const uint4 s0 = lds128(src + grp * 2176 + (it & 3) * 32), s1 = lds128(src + grp * 2176 + (it & 3) * 32 + 16);
-          const uint32_t qs[4] = {q.x, q.y, q.z, q.w}, sc[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
-          uint32_t o[8];
+        for (int grp = 0; grp < 2; ++grp) {
+          const int phys = grp ? sh.y : sh.x, off = grp ? sh.z >> 16 : sh.z & 0xffff;
+          sc[grp] = 0;
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            dequant4(qs[e], *reinterpret_cast<const __half2*>(&sc[2 * e]), *reinterpret_cast<const __half2*>(&sc[2 * e + 1]),
-                     o[2 * e], o[2 * e + 1]);
-          if (checked) {
-            const int nv = valid - 16 * grp;
+          for (int i = 0; i < 4; ++i) q[grp][i] = make_uint4(0, 0, 0, 0);
+          if (phys >= 0) {
+            const uint8_t* rec = vbase + (int64_t)phys * p.v_page_stride;
+            // word `lane`: scales of keys 2 * (lane % 8), + 1 of block lane / 8
+            sc[grp] = *reinterpret_cast<const uint32_t*>(rec + 2 * ((lane >> 3) * bsz + off) + 4 * (lane & 7));
 #pragma unroll
-            for (int e = 0; e < 8; ++e) hit |= clean2(o[e], 2 * e >= nv, 2 * e + 1 >= nv);
+            for (int i = 0; i < 4; ++i)
+              q[grp][i] = ldg16_early(rec + 2 * (D / QK) * bsz + (int64_t)(lane + 32 * i) * bsz + off);
           }
-          const int key = 32 * w + 16 * grp;
-          const uint32_t at = tile + (key >> 6) * (TILE / 2) + d * 128;
-          const int c = (key & 63) >> 3;
-          sts128(at + ((c ^ (d & 7)) << 4), o[0], o[1], o[2], o[3]);
-          sts128(at + (((c + 1) ^ (d & 7)) << 4), o[4], o[5], o[6], o[7]);
         }
+        if (t + 1 < N) convert_k(t + 1);
+        if (ok) wait_vempty(t);
+        if (!ok) break;
+#pragma unroll
+        for (int grp = 0; grp < 2; ++grp) vscale[32 * grp + lane] = sc[grp];
+        __syncwarp();
+#pragma unroll
+        for (int grp = 0; grp < 2; ++grp) {
+          const int key = 32 * w + 16 * grp, c = (key & 63) >> 3;
+          uint8_t* at = tile + (key >> 6) * (TILE / 2);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int d = lane + 32 * i;
+            const uint4 s0 = *reinterpret_cast<const uint4*>(&vscale[32 * grp + 8 * i]);
+            const uint4 s1 = *reinterpret_cast<const uint4*>(&vscale[32 * grp + 8 * i + 4]);
+            const uint32_t qs[4] = {q[grp][i].x, q[grp][i].y, q[grp][i].z, q[grp][i].w};
+            const uint32_t s8[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+            uint32_t o[8];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              dequant4(qs[e], *reinterpret_cast<const __half2*>(&s8[2 * e]), *reinterpret_cast<const __half2*>(&s8[2 * e + 1]),
+                       o[2 * e], o[2 * e + 1]);
+            *reinterpret_cast<uint4*>(at + d * 128 + ((c ^ (d & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+            *reinterpret_cast<uint4*>(at + d * 128 + (((c + 1) ^ (d & 7)) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
+          }
+        }
+        if (checked) {
+          // again over what this lane wrote: keys past the sequence, values that are not finite
+#pragma unroll 1
+          for (int i = 0; i < 16; ++i) {
+            const int d = lane + 32 * (i & 3), c8 = i >> 2, key = 32 * w + 8 * c8, nv = valid - 8 * c8;
+            uint4* at = reinterpret_cast<uint4*>(tile + (key >> 6) * (TILE / 2) + d * 128 + ((((key & 63) >> 3) ^ (d & 7)) << 4));
+            const uint4 x4 = *at;
+            uint32_t o[4] = {x4.x, x4.y, x4.z, x4.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) hit |= clean2(o[e], 2 * e >= nv, 2 * e + 1 >= nv);
+            *at = make_uint4(o[0], o[1], o[2], o[3]);
+          }
+        }
+        __syncwarp();                        // vscale is free again
       } else {
-        const int key = 32 * w + lane;
-        if constexpr (VF == G9_VFMT_Q8) convert_rows(src, tile, key);
+        if constexpr (DIRECT) {
+          // 16-bit rows go straight into the operand tile; rows of a page that is not there are zeroed
+          wait_vempty(t);
+          if (!ok) break;
+          const int c = lane & 15;
+#pragma unroll
+          for (int grp = 0; grp < 2; ++grp) {
+            const int phys = grp ? sh.y : sh.x, off = grp ? sh.z >> 16 : sh.z & 0xffff;
+            const uint8_t* src = vbase + (int64_t)phys * p.v_page_stride + (int64_t)off * p.v_tok_stride + 16 * c;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int r = 2 * i + (lane >> 4), key = 32 * w + 16 * grp + r;
+              uint8_t* at = tile + (c >> 3) * (TILE / 2) + key * 128 + (((c & 7) ^ (key & 7)) << 4);
+              if (phys >= 0) cp_async16(smem_u32(at), src + (int64_t)r * p.v_tok_stride);
+              else *reinterpret_cast<uint4*>(at) = make_uint4(0, 0, 0, 0);
+            }
+          }
+          cp_async_mbar_arrive(&vraw[w]);
+          if (t + 1 < N) convert_k(t + 1);
+          if (!ok || !mbar_wait(&vraw[w], t & 1)) { ok = false; break; }
+        } else {
+          if (t + 1 < N) convert_k(t + 1);
+          if (ok) wait_vempty(t);
+          if (!ok) break;
+#pragma unroll 1
+          for (int grp = 0; grp < 2; ++grp) {
+            const uint8_t* src = take();
+            convert_rows<0>(src, tile, 32 * w + 16 * grp);
+            release();
+          }
+        }
         // bf16 V becomes fp16 in place: exact for 2^-14 <= |v| < 65520, and P keeps fp16's 11 bits (in bf16 it would keep 8,
         // which rows of few keys show)
         if (VF == G9_VFMT_BF16 || checked) {
-          // own row: lane = key (token rows were written by this lane; 16-bit rows arrived by copies of this warp)
+          __syncwarp();
+          const int key = 32 * w + lane;
           const bool dead = lane >= valid;
+#pragma unroll 2
           for (int c = 0; c < 16; ++c) {
-            const uint32_t at = tile + (c >> 3) * (TILE / 2) + key * 128 + (((c & 7) ^ (key & 7)) << 4);
-            uint4 x4 = lds128(at);
+            uint4* at = reinterpret_cast<uint4*>(tile + (c >> 3) * (TILE / 2) + key * 128 + (((c & 7) ^ (key & 7)) << 4));
+            const uint4 x4 = *at;
             uint32_t o[4] = {x4.x, x4.y, x4.z, x4.w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -690,39 +647,55 @@ __global__ void __launch_bounds__(tt::NT, 1) tree_tc_kernel(const __grid_constan
                 o[e] = pack_half2(__uint_as_float(o[e] << 16), __uint_as_float(o[e] & 0xffff0000u));
               if (checked) hit |= clean2(o[e], dead, dead);
             }
-            sts128(at, o[0], o[1], o[2], o[3]);
+            *at = make_uint4(o[0], o[1], o[2], o[3]);
           }
         }
       }
       if (hit) misc[2] = 1;
-      fence_proxy_async();
       __syncwarp();
       if (lane == 0) mbar_arrive(&vfull[t & 1]);
-    };
-    for (int x = 0; ok && N > 0 && x < E - 1; ++x) {
-      if (x <= 2 * N) load_item(x);
-      cp_async_commit();
-    }
-    for (int x = 0; ok && N > 0 && x <= 2 * N; ++x) {
-      if (x + E - 1 <= 2 * N) load_item(x + E - 1);
-      if (!ok) break;
-      cp_async_commit();
-      cp_async_wait<E - 1>();
-      __syncwarp();
-      convert_item(x);
-      __syncwarp();
     }
     cp_async_wait<0>();
+    ok = __all_sync(0xffffffffu, ok);
     if (!ok) *abort_flag = 1;
   } else {
     // ======================= softmax streams =====================================
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REG_SOFT));
-    const int wi = (warp - 8) >> 2;          // stream
+    const int wi = warp >> 2;          // stream
     const int r = (warp & 3) * 32 + lane;    // row of the tile = TMEM lane
     const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t tS = tmem + wi * 128 + lane_off, tO = tmem + 256 + wi * 128 + lane_off;
     const bool general = p.softcap > 0.f || !(p.scale > 0.f);
-    int n0 = 0, ns = 0, cs = 0;              // tiles, segments, steps of this stream so far
+    const bool leader = (tid & 127) == 0;    // issues the stream's MMAs
+    constexpr uint32_t kS = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+    constexpr uint32_t kPV = kS | (VF == G9_VFMT_Q8T ? 0u : 1u << 16);        // V by token rows: N-major
+    const uint32_t qs = sQ + (NQ == 2 ? wi * TILE : 0);
+    // The proxy fence that lets the tensor core read what the loaders wrote stands here, after the wait for
+    // their arrivals, and not at their stores: there it would wait for their copies still in flight, a memory latency a tile.
+    // Descriptors are advanced from one base each: the start address counts 16-byte units in the low bits.
+    auto issue_s = [&](int n) {              // S = Q K(n)^T
+      fence_proxy_async();
+      const uint64_t qd = sw128_desc(qs), kd = sw128_desc(sK + (n & 1) * TILE);
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        const uint32_t off = ((kk >> 2) * (TILE / 2) + (kk & 3) * 32) >> 4;
+        tc_mma_ss(tmem + wi * 128, qd + off, kd + off, kS, kk > 0);
+      }
+      tc_commit(&bs_[wi]);
+      tc_commit(&kempty[n & 1]);
+    };
+    auto issue_pv = [&](int n, bool first) { // O += P V(n)
+      fence_proxy_async();
+      const uint32_t vs = sV + (n & 1) * TILE;
+      const uint64_t vd = VF == G9_VFMT_Q8T ? sw128_desc(vs) : sw128_desc_mn(vs, TILE / 2);
+#pragma unroll
+      for (int kk = 0; kk < BN / 16; ++kk) {
+        const uint32_t off = (VF == G9_VFMT_Q8T ? (kk >> 2) * (TILE / 2) + (kk & 3) * 32 : kk * 2048) >> 4;
+        tc_mma_ts(tmem + 256 + wi * 128, tmem + wi * 128 + kk * 8, vd + off, kPV, (!first || kk > 0) ? 1u : 0u);
+      }
+      tc_commit(&vempty[n & 1]);
+    };
+    constexpr int STEP = NQ == 1 ? 2 : 1;    // tiles between a stream's own
+    int n0 = 0, ns = 0, cs = 0, cq = 0;      // tiles, segments, steps and Q tiles of this stream so far
     bool alive = true;
     TreeSeg s;
     while (alive && walk.next(a, s)) {
@@ -734,23 +707,111 @@ __global__ void __launch_bounds__(tt::NT, 1) tree_tc_kernel(const __grid_constan
       const int lo = row_live ? tree_window_lo(a, bits, s.nq, s.ctx) : 0;
       float m = -INFINITY, l = 0.f;          // log2 units
       const bool stream_on = NQ == 1 || wi == 0 || s.rows > BM;
-      for (int j = NQ == 1 ? wi : 0; stream_on && j < s.n; j += NQ == 1 ? 2 : 1) {
-        if (!mbar_wait(&bs_[wi], cs & 1)) alive = false;
+      const int j0 = NQ == 1 ? wi : 0;
+      // ---- Q rows of this stream's tile (NQ = 1: half the columns each) -------------
+      // The previous segment's MMAs are done: every thread has waited for them.
+      if (stream_on || NQ == 1) {
+        constexpr int COLS = NQ == 1 ? 8 : 16;           // 16-byte pieces of a row
+        const int c0 = NQ == 1 ? 8 * wi : 0;
+#pragma unroll 4
+        for (int it = tid & 127; it < BM * COLS; it += 128) {
+          const int qr = it / COLS, c = c0 + it % COLS;
+          const int gr = (NQ == 2 ? wi * BM : 0) + qr;
+          uint32_t v[4] = {0, 0, 0, 0};
+          if (gr < s.rows) {
+            const int x = s.row0 + gr, xt = x / a.G;
+            const int64_t at = q_offset(p, s.b, xt, h * a.G + x - xt * a.G) + 8 * c;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              v[e] = pack_half2(load_one(p.q, at + 2 * e, p.q_dtype), load_one(p.q, at + 2 * e + 1, p.q_dtype));
+          }
+          sts128(qs + (c >> 3) * (TILE / 2) + qr * 128 + (((c & 7) ^ (qr & 7)) << 4), v[0], v[1], v[2], v[3]);
+        }
+        fence_proxy_async();
+        mbar_arrive(&qfull[NQ == 1 ? 0 : wi]);
+      }
+      if (leader) {
+        if (stream_on && j0 < s.n) {
+          alive = mbar_wait(&qfull[NQ == 1 ? 0 : wi], (NQ == 1 ? ns : cq) & 1) && mbar_wait(&kfull[(n0 + j0) & 1], ((n0 + j0) >> 1) & 1);
+          if (alive) {
+            tc_fence_after();
+            issue_s(n0 + j0);
+          }
+        } else {
+          mbar_arrive(&bo[wi]);              // nothing to multiply
+          if (NQ == 2)                       // pass this stream's share of every tile on
+            for (int j = 0; alive && j < s.n; ++j) {
+              alive = mbar_wait(&kfull[(n0 + j) & 1], ((n0 + j) >> 1) & 1);
+              mbar_arrive(&kempty[(n0 + j) & 1]);
+              alive = alive && mbar_wait(&vfull[(n0 + j) & 1], ((n0 + j) >> 1) & 1);
+              mbar_arrive(&vempty[(n0 + j) & 1]);
+            }
+        }
+      }
+      if (NQ == 2 && stream_on) ++cq;
+      // after a step's weights are in place: PV of this tile, then the scores of the stream's next one
+      auto multiply = [&](int j) {
+        if (!leader) return;
+        const int n = n0 + j;
+        alive = mbar_wait(&bp[wi], (cs - 1) & 1) && mbar_wait(&vfull[n & 1], (n >> 1) & 1);
+        if (!alive) return;
+        tc_fence_after();
+        issue_pv(n, j == j0);
+        if (j + STEP < s.n) {
+          alive = mbar_wait(&kfull[(n + STEP) & 1], ((n + STEP) >> 1) & 1);
+          if (!alive) return;
+          tc_fence_after();
+          issue_s(n + STEP);
+        } else {
+          tc_commit(&bo[wi]);
+        }
+      };
+      for (int j = j0; stream_on && j < s.n; j += STEP) {
+        if (alive && !mbar_wait(&bs_[wi], cs & 1)) alive = false;
         alive = __all_sync(0xffffffffu, alive);
         if (!alive) break;
         ++cs;
         tc_fence_after();
-        if (!warp_live) {
-          mbar_arrive(&bph[wi]);
-          mbar_arrive(&bp[wi]);
-          continue;
-        }
+        if (warp_live) {
         const int k0 = (s.j + j) * BN;
         const uint32_t bad = tilebad[(n0 + j) & 7];
         const bool checked = bad || tree_checked(a, s, k0);
+        // Scores that a cap or the mask changes are written back first, in small loops: code that most tiles skip must
+        // not stand between the instructions that every tile runs (the kernel was bound by instruction fetch).
+        if (general) {
+#pragma unroll 1
+          for (int c = 0; c < 16; ++c) {
+            uint32_t x[8];
+            tmem_ld8(tS + c * 8, x);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float y = __uint_as_float(x[e]);
+              x[e] = __float_as_uint(p.softcap > 0.f ? softcap_log2(y, a.cap_in, a.cap_out) : y * a.scale_log2);
+            }
+            tmem_st8(tS + c * 8, x);
+          }
+          tmem_wait_st();
+        }
+        if (checked) {
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            uint32_t x[32];
+            tmem_ld32(tS + c * 32, x);
+            tmem_wait_ld();
+            uint32_t v = row_live ? tree_sees(bits, a.words, s.nq, s.ctx, lo, k0 + 32 * c) : 0u;
+            const uint32_t bc = bad >> (8 * c);            // loader warp c holds keys 32c .. 32c + 31
+            if (bc & 1) v &= 0xffff0000u;
+            if (bc & 2) v &= 0x0000ffffu;
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (!(v >> e & 1u)) x[e] = 0xff800000u;
+            tmem_st32(tS + c * 32, x);
+          }
+          tmem_wait_st();
+        }
         // Two passes over the scores, 64 at a time, so that a row never holds
-        // all 128 in registers: the maximum first (scores that a cap or the
-        // mask changes are written back), then the weights.
+        // all 128 in registers: the maximum first, then the weights.
         float mx = -INFINITY;
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
@@ -758,31 +819,6 @@ __global__ void __launch_bounds__(tt::NT, 1) tree_tc_kernel(const __grid_constan
           tmem_ld32(tS + hf * 64, x[0]);
           tmem_ld32(tS + hf * 64 + 32, x[1]);
           tmem_wait_ld();
-          if (general) {
-#pragma unroll
-            for (int c = 0; c < 2; ++c)
-#pragma unroll
-              for (int e = 0; e < 32; ++e) {
-                const float y = __uint_as_float(x[c][e]);
-                x[c][e] = __float_as_uint(p.softcap > 0.f ? softcap_log2(y, a.cap_in, a.cap_out) : y * a.scale_log2);
-              }
-          }
-          if (checked) {
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              uint32_t v = row_live ? tree_sees(bits, a.words, s.nq, s.ctx, lo, k0 + 64 * hf + 32 * c) : 0u;
-              const uint32_t bc = bad >> (8 * (2 * hf + c));     // loader warp i holds keys 32i .. 32i + 31
-              if (bc & 1) v &= 0xffff0000u;
-              if (bc & 2) v &= 0x0000ffffu;
-#pragma unroll
-              for (int e = 0; e < 32; ++e)
-                if (!(v >> e & 1u)) x[c][e] = 0xff800000u;
-            }
-          }
-          if (general || checked) {
-            tmem_st32(tS + hf * 64, x[0]);
-            tmem_st32(tS + hf * 64 + 32, x[1]);
-          }
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             float m0 = __uint_as_float(x[c][0]), m1 = __uint_as_float(x[c][1]);
@@ -794,7 +830,6 @@ __global__ void __launch_bounds__(tt::NT, 1) tree_tc_kernel(const __grid_constan
             mx = fmax3(mx, fmax3(m0, m1, __uint_as_float(x[c][30])), __uint_as_float(x[c][31]));
           }
         }
-        if (general || checked) tmem_wait_st();
         if (!general) mx *= a.scale_log2;    // scale > 0: the maximum commutes with it
         float alpha = 1.f;
         bool rescale = false;
@@ -808,7 +843,7 @@ __global__ void __launch_bounds__(tt::NT, 1) tree_tc_kernel(const __grid_constan
         }
         if (__any_sync(0xffffffffu, rescale)) {
           // S(j) complete: every earlier PV of this stream is in O
-#pragma unroll
+#pragma unroll 1
           for (int c = 0; c < 4; ++c) {
             uint32_t o[32];
             tmem_ld32(tO + c * 32, o);
@@ -843,15 +878,7 @@ __global__ void __launch_bounds__(tt::NT, 1) tree_tc_kernel(const __grid_constan
               pk[e] = pack_half2(y0, y1);
             }
             // 64 weights take 32 columns: columns whose scores this row has read
-            asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
-                         ::"r"(tS + hf * 32 + c * 8), "r"(pk[0]), "r"(pk[1]), "r"(pk[2]), "r"(pk[3]), "r"(pk[4]), "r"(pk[5]),
-                           "r"(pk[6]), "r"(pk[7])
-                         : "memory");
-          }
-          if (hf == 0) {                     // half of P (and any rescaled O) is in place
-            tmem_wait_st();
-            tc_fence_before();
-            mbar_arrive(&bph[wi]);
+            tmem_st8(tS + hf * 32 + c * 8, pk);
           }
         }
         float a0, a1, b0, b1;
@@ -859,8 +886,10 @@ __global__ void __launch_bounds__(tt::NT, 1) tree_tc_kernel(const __grid_constan
         f2unpack(ls2[1], b0, b1);
         l += (a0 + a1) + (b0 + b1);
         tmem_wait_st();
+        }                                    // rows past the group keep whatever S holds: O's rows are apart
         tc_fence_before();
         mbar_arrive(&bp[wi]);
+        multiply(j);
       }
       // ---- the segment's rows ------------------------------------------------------
       if (l != l && m == -INFINITY) m = 0.f; // only NaN scores: the row is one too
@@ -870,7 +899,7 @@ __global__ void __launch_bounds__(tt::NT, 1) tree_tc_kernel(const __grid_constan
         stat[(wi * 2) * BM + r] = m;
         stat[(wi * 2 + 1) * BM + r] = l;
         mbar_arrive(bx);
-        if (!alive || !mbar_wait(bx, ns & 1)) alive = false;
+        if (alive && !mbar_wait(bx, ns & 1)) alive = false;
       }
       if (!alive || !mbar_wait(&bo[0], ns & 1) || !mbar_wait(&bo[1], ns & 1)) alive = false;
       alive = __all_sync(0xffffffffu, alive);
@@ -966,7 +995,7 @@ __global__ void __launch_bounds__(tt::NT, 1) tree_tc_kernel(const __grid_constan
   tc_fence_before();
   __syncthreads();
   if (tid == 0 && misc[1]) raise_error(ERR_WAIT_TIMEOUT);
-  if (warp == 1) {
+  if (warp == 8) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
   }
