@@ -872,6 +872,7 @@ torch::Tensor tree_attention(torch::Tensor query, torch::Tensor key_cache_q8, to
   const int64_t T = query.size(0), Hq = query.size(1), D = query.size(2), B = block_table.size(0);
   check_paged(key_cache_q8, value_cache, block_table, seq_lens, D, B);
   check_index(query_start_loc, "query_start_loc", torch::kInt32, B + 1);
+  TORCH_CHECK(key_cache_q8.size(0) > 0 && key_cache_q8.size(1) > 0, "the cache has no pages");
   TORCH_CHECK(Hq > 0 && key_cache_q8.size(2) > 0 && Hq % key_cache_q8.size(2) == 0, "heads_q must be divisible by heads_kv");
   TORCH_CHECK(tree_mask.device().is_cuda() && tree_mask.dtype() == torch::kInt32 && tree_mask.dim() == 2 &&
                   tree_mask.size(0) >= T && (tree_mask.size(1) <= 1 || tree_mask.stride(1) == 1),

@@ -174,7 +174,7 @@ TreePlan plan_tree(const G9AttnBatch& p) {
   auto off = [](uintptr_t base, int64_t a, int64_t b, int64_t c, uintptr_t to) {
     return ((base | (uintptr_t)a | (uintptr_t)b | (uintptr_t)c) & (to - 1)) != 0;
   };
-  if (p.block_size % 16) return pl;
+  if (p.block_size % 16 || p.max_blocks == 0) return pl;
   if (off((uintptr_t)p.k_cache, p.k_page_stride, p.k_tok_stride, p.k_head_stride, 8)) return pl;
   const uintptr_t va = p.v_fmt == G9_VFMT_Q8 ? 8 : 16;
   if (off((uintptr_t)p.v_cache, p.v_page_stride, p.v_fmt == G9_VFMT_Q8T ? 0 : p.v_tok_stride, p.v_head_stride, va)) return pl;

@@ -243,7 +243,12 @@ __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_gr
 // arrives on `bar` when this thread's copies so far have landed
 __device__ __forceinline__ void cp_async_mbar_arrive(uint64_t* bar) { cp_async_arrive_noinc(bar); }
 
-// a load that stays where it is written, ahead of the work that hides it
+// loads that stay where they are written, ahead of the work that hides them
+__device__ __forceinline__ uint32_t ldg4_early(const void* p) {
+  uint32_t v;
+  asm volatile("ld.global.L1::no_allocate.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
 __device__ __forceinline__ uint4 ldg16_early(const void* p) {
   uint4 v;
   asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
@@ -419,8 +424,9 @@ __global__ void __launch_bounds__(tt::NT, 1) tree_tc_kernel(const __grid_constan
       const int k = key0 + 32 * w;
       const int32_t* bt = p.block_table + (int64_t)s.b * p.max_blocks;
       const int pg0 = k / bsz, pg1 = (k + 16) / bsz;
-      ph0 = k < s.L ? bt[pg0] : -1;
-      ph1 = k + 16 < s.L ? bt[pg1] : -1;
+      // no branch around a load that is meant to stay in flight: joining its result with another value waits for it
+      ph0 = bt[min(pg0, p.max_blocks - 1)];
+      ph1 = bt[min(pg1, p.max_blocks - 1)];
       of0 = k - pg0 * bsz;
       of1 = k + 16 - pg1 * bsz;
       info = max(0, min(32, s.L - k)) | (tree_checked(a, s, key0) ? 256 : 0);
@@ -431,8 +437,10 @@ __global__ void __launch_bounds__(tt::NT, 1) tree_tc_kernel(const __grid_constan
     // notes what the last lookup brought
     auto settle = [&]() {
       uint32_t bad = 0;                      // groups with keys on a page that is not there
-      if ((info & 0xff) > 0 && page_bad(p, ph0)) { bad |= 1; ph0 = -1; }
-      if ((info & 0xff) > 16 && page_bad(p, ph1)) { bad |= 2; ph1 = -1; }
+      if ((info & 0xff) == 0) ph0 = -1;
+      else if (page_bad(p, ph0)) { bad |= 1; ph0 = -1; }
+      if ((info & 0xff) <= 16) ph1 = -1;
+      else if (page_bad(p, ph1)) { bad |= 2; ph1 = -1; }
       if (bad) {
         info |= 256;
         if (lane == 0) raise_error(ERR_BAD_PAGE);
@@ -546,23 +554,19 @@ __global__ void __launch_bounds__(tt::NT, 1) tree_tc_kernel(const __grid_constan
 #pragma unroll
         for (int grp = 0; grp < 2; ++grp) {
           const int phys = grp ? sh.y : sh.x, off = grp ? sh.z >> 16 : sh.z & 0xffff;
-          sc[grp] = 0;
+          // a page that is not there: page 0's bytes with scales of zero
+          const uint8_t* rec = vbase + (int64_t)max(phys, 0) * p.v_page_stride;
+          const int at = phys < 0 ? 0 : off;
+          // word `lane`: scales of keys 2 * (lane % 8), + 1 of block lane / 8
+          sc[grp] = ldg4_early(rec + 2 * ((lane >> 3) * bsz + at) + 4 * (lane & 7));
 #pragma unroll
-          for (int i = 0; i < 4; ++i) q[grp][i] = make_uint4(0, 0, 0, 0);
-          if (phys >= 0) {
-            const uint8_t* rec = vbase + (int64_t)phys * p.v_page_stride;
-            // word `lane`: scales of keys 2 * (lane % 8), + 1 of block lane / 8
-            sc[grp] = *reinterpret_cast<const uint32_t*>(rec + 2 * ((lane >> 3) * bsz + off) + 4 * (lane & 7));
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              q[grp][i] = ldg16_early(rec + 2 * (D / QK) * bsz + (int64_t)(lane + 32 * i) * bsz + off);
-          }
+          for (int i = 0; i < 4; ++i) q[grp][i] = ldg16_early(rec + 2 * (D / QK) * bsz + (int64_t)(lane + 32 * i) * bsz + at);
         }
         if (t + 1 < N) convert_k(t + 1);
         if (ok) wait_vempty(t);
         if (!ok) break;
 #pragma unroll
-        for (int grp = 0; grp < 2; ++grp) vscale[32 * grp + lane] = sc[grp];
+        for (int grp = 0; grp < 2; ++grp) vscale[32 * grp + lane] = (grp ? sh.y : sh.x) < 0 ? 0u : sc[grp];
         __syncwarp();
 #pragma unroll
         for (int grp = 0; grp < 2; ++grp) {
