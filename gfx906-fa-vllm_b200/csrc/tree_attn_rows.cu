@@ -231,6 +231,9 @@ extern "C" cudaError_t gfx906_fa_tree_attention(const G9AttnBatch* batch, const 
   pp.Hkv = batch->num_heads_kv;
   pp.NG = pl.NG;
   pp.rc = pl.rc;
+  pp.bs_log2 = -1;
+  if ((batch->block_size & (batch->block_size - 1)) == 0)
+    for (pp.bs_log2 = 0; (1 << pp.bs_log2) < batch->block_size;) ++pp.bs_log2;
   // Rows of odd heads start 8 bytes off a 16-byte boundary and take the 8 bytes before them along; those of even heads the 8
   // behind them, which the next head's row holds.
   pp.k_wide = (((uintptr_t)batch->k_cache | (uintptr_t)batch->k_page_stride | (uintptr_t)batch->k_tok_stride) & 15) == 0 &&

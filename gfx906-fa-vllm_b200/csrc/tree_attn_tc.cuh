@@ -16,15 +16,16 @@
 // the same number of tiles whatever the lengths.  An item cut by a range border
 // leaves partial rows that tree_combine_kernel joins.
 //
-// CTA, 12 warps of 168 registers (16 warps hold 128 each, where the loaders and
-// the softmax spill, and L1 is too small beside 227 KB of shared memory for
-// what they spill):
+// CTA:
 //   warps 0-7    two softmax streams, a thread a row (row = TMEM lane).  A stream's first thread
 //                also issues its tcgen05.mma: the stream has nothing else to do until its next
 //                scores are there, so no warp is spent on it.
-//   warps 8-11   load cache rows and convert: K to [key][d], V to [d][key] (page-transposed Q8_0)
-//                or [key][d] (token rows); a warp owns 32 keys of a tile, so loading and converting
-//                need no barrier between warps
+//   warps 8-     loaders, groups of four warps that take key tiles in turn: they load cache rows
+//                and convert them, K to [key][d], V to [d][key] (page-transposed Q8_0) or [key][d]
+//                (token rows).  A warp owns 32 keys of its tiles, so loading and converting need no
+//                barrier between warps.  NQ = 1 has two groups (16 warps of 128 registers): one
+//                warp a scheduler leaves it idle through its latencies and instruction fetches.
+//                NQ = 2, whose softmax is twice the work per key, has one (12 warps of 168).
 // One query tile (NQ = 1): the streams take alternate key tiles of the same
 // rows, each with its own running maximum, sum and accumulator, so that one
 // stream's softmax runs under the other's MMAs; they are joined through TMEM at
@@ -45,17 +46,16 @@ constexpr int BM = 128;
 constexpr int BN = 128;
 constexpr int ST = 2;                        // K and V stages
 constexpr int TILE = BM * D * 2;             // 32 KB
-constexpr int NT = 384;
 constexpr int PITCH = 144;                   // raw Q8_0 rows: 136 bytes, up to 8 before or behind them
-constexpr int RAW = 16 * PITCH;              // a warp's slot: 16 raw rows
+constexpr int RAW = 32 * PITCH;              // a warp's 32 raw rows
+constexpr int loader_groups(int nq) { return nq == 1 ? 2 : 1; }
+constexpr int threads(int nq) { return 256 + 128 * loader_groups(nq); }
 constexpr float kRescale = 8.0f;             // log2 units
 
-// raw slots a warp rotates through, in the shared memory that the tiles leave
-constexpr int raw_slots(int nq) { return nq == 1 ? 7 : 3; }
 constexpr int smem_raw_off(int nq) { return (2 * ST + nq) * TILE; }
-constexpr int smem_stat_off(int nq) { return smem_raw_off(nq) + raw_slots(nq) * 4 * RAW; }
-constexpr int smem_share_off(int nq) { return smem_stat_off(nq) + (nq == 1 ? 2 * 2 * BM * 4 : 0); }
-constexpr int smem_bar_off(int nq) { return smem_share_off(nq) + 4 * 8 * 16 + 4 * 256; }
+constexpr int smem_stat_off(int nq) { return smem_raw_off(nq) + 4 * loader_groups(nq) * RAW; }
+constexpr int smem_scale_off(int nq) { return smem_stat_off(nq) + (nq == 1 ? 2 * 2 * BM * 4 : 0); }
+constexpr int smem_bar_off(int nq) { return smem_scale_off(nq) + 4 * loader_groups(nq) * 256; }
 constexpr int smem_bytes(int nq) { return smem_bar_off(nq) + 512; }
 static_assert(smem_bytes(1) <= 232448 && smem_bytes(2) <= 232448, "shared memory");
 }  // namespace tt
@@ -64,6 +64,7 @@ struct TreeTcParams {
   TreeArgs a;
   int Hkv, NG;
   int rc;                        // rows of a partial block (a multiple of 32)
+  int bs_log2;                   // of the page size, -1: not a power of two
   int k_wide;                    // K rows may be copied as 16-byte pieces (even head counts)
   int out_vec;                   // output rows may be written 16 bytes at a time
   int* cum;                      // [num_seqs + 1] first unit of each sequence
@@ -239,16 +240,13 @@ __device__ __forceinline__ void cp_async8(uint32_t dst, const void* src) {
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
-// arrives on `bar` when this thread's copies so far have landed
-__device__ __forceinline__ void cp_async_mbar_arrive(uint64_t* bar) { cp_async_arrive_noinc(bar); }
-
 // loads that stay where they are written, ahead of the work that hides them
 __device__ __forceinline__ uint32_t ldg4_early(const void* p) {
   uint32_t v;
   asm volatile("ld.global.L1::no_allocate.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
   return v;
 }
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 __device__ __forceinline__ uint4 ldg16_early(const void* p) {
   uint4 v;
   asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
@@ -295,9 +293,9 @@ __device__ __forceinline__ void convert_rows(const uint8_t* raw, uint8_t* tile, 
 
 // ===========================================================================
 template <int NQ, int VF>
-__global__ void __launch_bounds__(tt::NT, 1) tree_tc_kernel(const __grid_constant__ TreeTcParams pp) {
+__global__ void __launch_bounds__(tt::threads(NQ), 1) tree_tc_kernel(const __grid_constant__ TreeTcParams pp) {
   using namespace tt;
-  constexpr int E = raw_slots(NQ);
+  constexpr int NT = threads(NQ), GROUPS = loader_groups(NQ);
   constexpr bool DIRECT = VF == G9_VFMT_F16 || VF == G9_VFMT_BF16;
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t sbase = smem_u32(smem);
@@ -306,8 +304,8 @@ __global__ void __launch_bounds__(tt::NT, 1) tree_tc_kernel(const __grid_constan
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + smem_bar_off(NQ));
   uint64_t *kfull = bars, *kempty = bars + 2, *vfull = bars + 4, *vempty = bars + 6, *qfull = bars + 8, *bs_ = bars + 10,
            *bp = bars + 12, *bo = bars + 14, *bx = bars + 16, *by = bars + 17, *vraw = bars + 18;
-  int* misc = reinterpret_cast<int*>(bars + 24);     // 0: tensor memory, 1: abort, 2: poison, 3: total, 4: b, 5: base, 8..23: scan
-  uint32_t* tilebad = reinterpret_cast<uint32_t*>(misc + 24);                // [8], a byte per loader warp
+  int* misc = reinterpret_cast<int*>(bars + 26);     // 0: tensor memory, 1: abort, 2: poison, 4: b, 5: base, 8..23: scan
+  uint32_t* tilebad = reinterpret_cast<uint32_t*>(misc + 24);                // [8], a byte per 32 keys
 
   const TreeArgs& a = pp.a;
   const G9AttnBatch& p = a.p;
@@ -322,7 +320,7 @@ __global__ void __launch_bounds__(tt::NT, 1) tree_tc_kernel(const __grid_constan
       mbar_init(&bs_[i], 1); mbar_init(&bp[i], 128); mbar_init(&bo[i], 1);
       mbar_init(&qfull[i], NQ == 1 ? 256 : 128);
     }
-    for (int i = 0; i < 4; ++i) mbar_init(&vraw[i], 32);
+    for (int i = 0; i < 4 * GROUPS; ++i) mbar_init(&vraw[i], 32);
     mbar_init(bx, 256); mbar_init(by, 256);
     misc[1] = misc[2] = 0;
     fence_barrier_init();
@@ -391,259 +389,229 @@ __global__ void __launch_bounds__(tt::NT, 1) tree_tc_kernel(const __grid_constan
 
   if (warp >= 8) {
     // ======================= cache rows: load and convert ========================
-    const int w = warp - 8;
+    const int lw = warp - 8, w = lw & 3;     // this warp's 32 keys of a tile
     const int bsz = p.block_size;
-    uint8_t* raw = smem + smem_raw_off(NQ) + w * E * RAW;      // this warp's slots
-    // pages of the last 8 tiles looked up: (page, offset) of the two 16-key groups, keys inside the sequence | checked << 8
-    int4* shares = reinterpret_cast<int4*>(smem + smem_share_off(NQ)) + 8 * w;
-    uint32_t* vscale = reinterpret_cast<uint32_t*>(smem + smem_share_off(NQ) + 4 * 8 * 16 + w * 256);
+    uint8_t* raw = smem + smem_raw_off(NQ) + lw * RAW;
+    uint32_t* vscale = reinterpret_cast<uint32_t*>(smem + smem_scale_off(NQ) + lw * 256);
     const int odd = pp.k_wide && (h & 1);    // the row starts 8 bytes into its first 16-byte piece
     const uint8_t* kbase = p.k_cache + (int64_t)h * p.k_head_stride - 8 * odd;
     const uint8_t* vbase = p.v_cache + (int64_t)h * p.v_head_stride;
-    // offsets of this lane's pieces of 16 token rows: 9 pieces of 16 bytes a row, or 17 of 8
-    int koff[5], kdst[5];
+    int koff[9];                             // this lane's pieces of 32 rows: nine of 16 bytes a row
 #pragma unroll
-    for (int i = 0; i < 5; ++i) {
-      const int x = i * 32 + lane, r = x / 9;
-      koff[i] = (int)(r * p.k_tok_stride) + (x - r * 9) * 16;
-      kdst[i] = r * PITCH + (x - r * 9) * 16;
+    for (int i = 0; i < 9; ++i) {
+      const int y = i * 32 + lane, r = y / 9;
+      koff[i] = (int)((r & 15) * p.k_tok_stride) + (y - r * 9) * 16;
     }
     TreeSeg s;
-    int left = 0, key0 = 0;                  // tiles left in the segment, first key of the next tile
-    int looked = 0;                          // tiles looked up
-    int ph0 = -1, ph1 = -1, of0 = 0, of1 = 0, info = 0;        // the last of them
+    s.n = 0;
+    int pos = lw >> 2;                       // the next tile's place in the segment
+    // This warp's share of a tile: pages and in-page offsets of its two 16-key groups (page -1: none), keys inside the
+    // sequence | checked << 8.
+    struct Share { int ph0, ph1, of0, of1, info; };
+    Share cur{-1, -1, 0, 0, 0}, nxt = cur;
     bool ok = true;
-    // asks for the next tile's pages; nothing here waits for them
+    // Asks for the next tile's pages; nothing here waits for them.  No branch around a load that is meant to stay in
+    // flight: joining its result with another value waits for it.
     auto lookup = [&]() {
-      if (looked >= N) return;
-      if (left == 0) {
+      while (pos >= s.n) {
+        pos -= s.n;
         if (!walk.next(a, s)) return;
-        left = s.n;
-        key0 = s.j * BN;
       }
-      const int k = key0 + 32 * w;
+      const int k = (s.j + pos) * BN + 32 * w;
+      const int pg0 = pp.bs_log2 >= 0 ? k >> pp.bs_log2 : k / bsz, pg1 = pp.bs_log2 >= 0 ? (k + 16) >> pp.bs_log2 : (k + 16) / bsz;
       const int32_t* bt = p.block_table + (int64_t)s.b * p.max_blocks;
-      const int pg0 = k / bsz, pg1 = (k + 16) / bsz;
-      // no branch around a load that is meant to stay in flight: joining its result with another value waits for it
-      ph0 = bt[min(pg0, p.max_blocks - 1)];
-      ph1 = bt[min(pg1, p.max_blocks - 1)];
-      of0 = k - pg0 * bsz;
-      of1 = k + 16 - pg1 * bsz;
-      info = max(0, min(32, s.L - k)) | (tree_checked(a, s, key0) ? 256 : 0);
-      --left;
-      key0 += BN;
-      ++looked;
+      nxt.ph0 = bt[min(pg0, p.max_blocks - 1)];
+      nxt.ph1 = bt[min(pg1, p.max_blocks - 1)];
+      nxt.of0 = k - pg0 * bsz;
+      nxt.of1 = k + 16 - pg1 * bsz;
+      nxt.info = max(0, min(32, s.L - k)) | (tree_checked(a, s, k - 32 * w) ? 256 : 0);
+      pos += GROUPS;
     };
-    // notes what the last lookup brought
-    auto settle = [&]() {
-      uint32_t bad = 0;                      // groups with keys on a page that is not there
-      if ((info & 0xff) == 0) ph0 = -1;
-      else if (page_bad(p, ph0)) { bad |= 1; ph0 = -1; }
-      if ((info & 0xff) <= 16) ph1 = -1;
-      else if (page_bad(p, ph1)) { bad |= 2; ph1 = -1; }
-      if (bad) {
-        info |= 256;
-        if (lane == 0) raise_error(ERR_BAD_PAGE);
+    // what the last lookup brought; t: its tile
+    auto settle = [&](int t) {
+      cur = nxt;
+      const int valid = cur.info & 0xff;
+      uint32_t bad = 0;                      // keys on a page that is not there
+      if (valid > 0 && page_bad(p, cur.ph0)) bad = 1;
+      if (valid > 16 && page_bad(p, cur.ph1)) bad |= 2;
+      if (valid <= 16 || bad) {              // not every tile
+        if (valid == 0 || (bad & 1)) cur.ph0 = -1;
+        if (valid <= 16 || (bad & 2)) cur.ph1 = -1;
+        if (bad) {
+          cur.info |= 256;
+          if (lane == 0) raise_error(ERR_BAD_PAGE);
+        }
       }
-      const int t = looked - 1;
-      if (lane == 0) {
-        reinterpret_cast<uint8_t*>(&tilebad[t & 7])[w] = (uint8_t)bad;
-        shares[t & 7] = make_int4(ph0, ph1, of0 | of1 << 16, info);
-      }
-      __syncwarp();
+      if (lane == 0) reinterpret_cast<uint8_t*>(&tilebad[t & 7])[w] = (uint8_t)bad;
     };
-    // 16 token rows of 136 bytes into a raw slot; stale rows of a page that is not there are masked or cleared later
-    auto load_rows = [&](uint32_t dst, const uint8_t* src, int64_t tok_stride, bool wide) {
+    // 32 token rows of 136 bytes into the raw slot.  A page that is not there: page 0's bytes, whose scores are masked
+    // and whose values are cleared.
+    auto load_rows = [&](const uint8_t* base, int64_t page_stride, int64_t tok_stride, bool wide) {
+      const uint8_t* s0 = base + (int64_t)max(cur.ph0, 0) * page_stride + (int64_t)(cur.ph0 < 0 ? 0 : cur.of0) * tok_stride;
+      const uint8_t* s1 = base + (int64_t)max(cur.ph1, 0) * page_stride + (int64_t)(cur.ph1 < 0 ? 0 : cur.of1) * tok_stride;
+      const uint32_t dst = smem_u32(raw) + lane * 16;
       if (wide) {
+        // pieces 0..143 are the first group's rows
 #pragma unroll
-        for (int i = 0; i < 5; ++i)
-          if (i < 4 || lane < 16) cp_async16(dst + kdst[i], src + koff[i]);
+        for (int i = 0; i < 9; ++i) cp_async16(dst + i * 512, (i < 4 || (i == 4 && lane < 16) ? s0 : s1) + koff[i]);
       } else {
-#pragma unroll 3
-        for (int x = lane; x < 272; x += 32) {
-          const int r = x / 17, c = x - r * 17;
-          cp_async8(dst + r * PITCH + c * 8, src + r * tok_stride + c * 8);
+#pragma unroll 2
+        for (int y = lane; y < 544; y += 32) {
+          const int r = y / 17, c = y - r * 17;
+          cp_async8(smem_u32(raw) + r * PITCH + c * 8, (r < 16 ? s0 : s1) + (r & 15) * tok_stride + c * 8);
         }
       }
     };
-    // The raw queue holds 16-row groups in the order they are converted: K of
-    // tile 0, then K of tile n + 1 and (token-row V) V of tile n.
-    constexpr int PER = VF == G9_VFMT_Q8 ? 4 : 2;              // groups a tile
-    const int groups = PER * N;
-    int issued = 0, taken = 0;
-    auto issue = [&]() {
-      if (issued < groups) {
-        // which tile, which operand
-        int t, isv = 0, grp;
-        if (PER == 2) {
-          t = issued >> 1;
-          grp = issued & 1;
-        } else if (issued < 2) {
-          t = 0;
-          grp = issued;
-        } else {
-          const int y = issued - 2, n = y >> 2;                // K(n + 1) two groups, V(n) two groups; the last tile has V only
-          const bool last = n == N - 1;
-          grp = y & 1;
-          isv = last || (y & 2);
-          t = isv ? n : n + 1;
-        }
-        if (!isv && grp == 0) {              // a new tile: its pages were asked for a tile ago
-          settle();
-          lookup();
-        }
-        const int4 sh = shares[t & 7];
-        const int phys = grp ? sh.y : sh.x, off = grp ? sh.z >> 16 : sh.z & 0xffff;
-        if (phys >= 0) {
-          const uint32_t dst = smem_u32(raw + (issued % E) * RAW);
-          if (!isv) load_rows(dst, kbase + (int64_t)phys * p.k_page_stride + (int64_t)off * p.k_tok_stride, p.k_tok_stride, pp.k_wide);
-          else load_rows(dst, vbase + (int64_t)phys * p.v_page_stride + (int64_t)off * p.v_tok_stride, p.v_tok_stride, false);
-        }
-        ++issued;
-      }
+    // K rows of the settled tile; its V, needed a little later, on its way into L2
+    auto load_k = [&]() {
+      load_rows(kbase, p.k_page_stride, p.k_tok_stride, pp.k_wide);
       cp_async_commit();
+      const int ph = lane < 16 ? cur.ph0 : cur.ph1, of = lane < 16 ? cur.of0 : cur.of1;
+      const uint8_t* rec = vbase + (int64_t)max(ph, 0) * p.v_page_stride;
+      const int at = ph < 0 ? 0 : of;
+      if constexpr (VF == G9_VFMT_Q8T) prefetch_l2(rec + at + (lane & 15) * 136);      // a 16-token page's record
+      else {
+        prefetch_l2(rec + (int64_t)(at + (lane & 15)) * p.v_tok_stride);
+        if (DIRECT) prefetch_l2(rec + (int64_t)(at + (lane & 15)) * p.v_tok_stride + 128);
+      }
     };
-    // the oldest group has arrived
-    auto take = [&]() -> const uint8_t* {
-      cp_async_wait<E - 2>();
-      __syncwarp();
-      return raw + (taken % E) * RAW;
-    };
-    auto release = [&]() {
-      __syncwarp();                          // every lane has read the slot
-      ++taken;
-      issue();
-    };
-    auto convert_k = [&](int t) {
-      if (t >= ST && !mbar_wait(&kempty[t & 1], ((t >> 1) - 1) & 1)) ok = false;
+    auto wait_empty = [&](uint64_t* bar, int t) {
+      if (t >= ST && !mbar_wait(&bar[t & 1], ((t >> 1) - 1) & 1)) ok = false;
       ok = __all_sync(0xffffffffu, ok);
-      if (!ok) return;
-      uint8_t* tile = smem + (t & 1) * TILE;
+      return ok;
+    };
+    auto convert = [&](uint8_t* tile, int shift) {
 #pragma unroll 1
       for (int grp = 0; grp < 2; ++grp) {
-        const uint8_t* src = take();
-        if (odd) convert_rows<1>(src, tile, 32 * w + 16 * grp);
-        else convert_rows<0>(src, tile, 32 * w + 16 * grp);
-        release();
+        if (shift) convert_rows<1>(raw + grp * 16 * PITCH, tile, 32 * w + 16 * grp);
+        else convert_rows<0>(raw + grp * 16 * PITCH, tile, 32 * w + 16 * grp);
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&kfull[t & 1]);
     };
-    auto wait_vempty = [&](int t) {
-      if (t >= ST && !mbar_wait(&vempty[t & 1], ((t >> 1) - 1) & 1)) ok = false;
-      ok = __all_sync(0xffffffffu, ok);
-    };
-    if (N > 0) {
+    if ((lw >> 2) < N) {
       lookup();
-#pragma unroll 1
-      for (int i = 0; i < E - 1; ++i) issue();
-      convert_k(0);
+      settle(lw >> 2);
+      load_k();
     }
 #pragma unroll 1
-    for (int t = 0; ok && t < N; ++t) {
-      const int4 sh = shares[t & 7];
-      const int valid = sh.w & 0xff;         // keys of this warp inside the sequence
-      const bool checked = (sh.w & 256) != 0;
-      uint8_t* tile = smem + (ST + (t & 1)) * TILE;
-      int hit = 0;
+    for (int t = lw >> 2; ok && t < N; t += GROUPS) {
+      // `cur` is tile t; its K rows are on their way
+      const Share me = cur;
+      const int valid = me.info & 0xff;      // keys of this warp inside the sequence
+      const bool checked = (me.info & 256) != 0;
+      const bool more = t + GROUPS < N;
+      uint8_t* vtile = smem + (ST + (t & 1)) * TILE;
+      uint4 q[2][4];
+      uint32_t sc[2];
       if constexpr (VF == G9_VFMT_Q8T) {
-        // Page-transposed records go through registers: a lane's 16 bytes are 16
-        // keys of one dim.  They are asked for before the next K tile is converted.
-        uint4 q[2][4];
-        uint32_t sc[2];
+        // Page-transposed records go through registers: a lane's 16 bytes are 16 keys of one dim.
+        // Scale word `lane`: keys 2 * (lane % 8), + 1 of block lane / 8.
 #pragma unroll
         for (int grp = 0; grp < 2; ++grp) {
-          const int phys = grp ? sh.y : sh.x, off = grp ? sh.z >> 16 : sh.z & 0xffff;
-          // a page that is not there: page 0's bytes with scales of zero
-          const uint8_t* rec = vbase + (int64_t)max(phys, 0) * p.v_page_stride;
-          const int at = phys < 0 ? 0 : off;
-          // word `lane`: scales of keys 2 * (lane % 8), + 1 of block lane / 8
+          const int ph = grp ? me.ph1 : me.ph0, at = ph < 0 ? 0 : grp ? me.of1 : me.of0;
+          const uint8_t* rec = vbase + (int64_t)max(ph, 0) * p.v_page_stride;
           sc[grp] = ldg4_early(rec + 2 * ((lane >> 3) * bsz + at) + 4 * (lane & 7));
 #pragma unroll
           for (int i = 0; i < 4; ++i) q[grp][i] = ldg16_early(rec + 2 * (D / QK) * bsz + (int64_t)(lane + 32 * i) * bsz + at);
         }
-        if (t + 1 < N) convert_k(t + 1);
-        if (ok) wait_vempty(t);
-        if (!ok) break;
-#pragma unroll
-        for (int grp = 0; grp < 2; ++grp) vscale[32 * grp + lane] = (grp ? sh.y : sh.x) < 0 ? 0u : sc[grp];
-        __syncwarp();
+      } else if constexpr (DIRECT) {
+        // 16-bit rows go straight into the operand tile; rows of a page that is not there are zeroed
+        if (!wait_empty(vempty, t)) break;
+        const int c = lane & 15;
 #pragma unroll
         for (int grp = 0; grp < 2; ++grp) {
-          const int key = 32 * w + 16 * grp, c = (key & 63) >> 3;
-          uint8_t* at = tile + (key >> 6) * (TILE / 2);
+          const int ph = grp ? me.ph1 : me.ph0, at = grp ? me.of1 : me.of0;
+          const uint8_t* src = vbase + (int64_t)ph * p.v_page_stride + (int64_t)at * p.v_tok_stride + 16 * c;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int r = 2 * i + (lane >> 4), key = 32 * w + 16 * grp + r;
+            uint8_t* to = vtile + (c >> 3) * (TILE / 2) + key * 128 + (((c & 7) ^ (key & 7)) << 4);
+            if (ph >= 0) cp_async16(smem_u32(to), src + (int64_t)r * p.v_tok_stride);
+            else *reinterpret_cast<uint4*>(to) = make_uint4(0, 0, 0, 0);
+          }
+        }
+        cp_async_arrive_noinc(&vraw[lw]);
+        cp_async_commit();
+      }
+      if (more) lookup();
+      // ---- K ------------------------------------------------------------------------
+      cp_async_wait<DIRECT ? 1 : 0>();
+      __syncwarp();
+      if (!wait_empty(kempty, t)) break;
+      convert(smem + (t & 1) * TILE, odd);
+      if (lane == 0) mbar_arrive(&kfull[t & 1]);
+      if (VF == G9_VFMT_Q8) {                // token-row V takes the slot in turn
+        load_rows(vbase, p.v_page_stride, p.v_tok_stride, false);
+        cp_async_commit();
+      } else if (more) {
+        settle(t + GROUPS);
+        load_k();
+      }
+      // ---- V ------------------------------------------------------------------------
+      int hit = 0;
+      if constexpr (VF == G9_VFMT_Q8T) {
+        if (!wait_empty(vempty, t)) break;
+        vscale[lane] = me.ph0 < 0 ? 0u : sc[0];
+        vscale[32 + lane] = me.ph1 < 0 ? 0u : sc[1];
+        __syncwarp();
+        uint8_t* to = vtile + (w >> 1) * (TILE / 2);       // this warp's half tile
+        const int c0 = (w & 1) * 4;                        // and its first 8-key chunk there
+#pragma unroll
+        for (int grp = 0; grp < 2; ++grp) {
+          const int c = c0 + 2 * grp;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int d = lane + 32 * i;
             const uint4 s0 = *reinterpret_cast<const uint4*>(&vscale[32 * grp + 8 * i]);
-            const uint4 s1 = *reinterpret_cast<const uint4*>(&vscale[32 * grp + 8 * i + 4]);
+            const uint4 s4 = *reinterpret_cast<const uint4*>(&vscale[32 * grp + 8 * i + 4]);
             const uint32_t qs[4] = {q[grp][i].x, q[grp][i].y, q[grp][i].z, q[grp][i].w};
-            const uint32_t s8[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+            const uint32_t s8[8] = {s0.x, s0.y, s0.z, s0.w, s4.x, s4.y, s4.z, s4.w};
             uint32_t o[8];
 #pragma unroll
             for (int e = 0; e < 4; ++e)
               dequant4(qs[e], *reinterpret_cast<const __half2*>(&s8[2 * e]), *reinterpret_cast<const __half2*>(&s8[2 * e + 1]),
                        o[2 * e], o[2 * e + 1]);
-            *reinterpret_cast<uint4*>(at + d * 128 + ((c ^ (d & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
-            *reinterpret_cast<uint4*>(at + d * 128 + (((c + 1) ^ (d & 7)) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
+            *reinterpret_cast<uint4*>(to + d * 128 + ((c ^ (d & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+            *reinterpret_cast<uint4*>(to + d * 128 + (((c + 1) ^ (d & 7)) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
           }
         }
         if (checked) {
           // again over what this lane wrote: keys past the sequence, values that are not finite
 #pragma unroll 1
           for (int i = 0; i < 16; ++i) {
-            const int d = lane + 32 * (i & 3), c8 = i >> 2, key = 32 * w + 8 * c8, nv = valid - 8 * c8;
-            uint4* at = reinterpret_cast<uint4*>(tile + (key >> 6) * (TILE / 2) + d * 128 + ((((key & 63) >> 3) ^ (d & 7)) << 4));
-            const uint4 x4 = *at;
+            const int d = lane + 32 * (i & 3), nv = valid - 8 * (i >> 2);
+            uint4* x = reinterpret_cast<uint4*>(to + d * 128 + (((c0 + (i >> 2)) ^ (d & 7)) << 4));
+            const uint4 x4 = *x;
             uint32_t o[4] = {x4.x, x4.y, x4.z, x4.w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) hit |= clean2(o[e], 2 * e >= nv, 2 * e + 1 >= nv);
-            *at = make_uint4(o[0], o[1], o[2], o[3]);
+            *x = make_uint4(o[0], o[1], o[2], o[3]);
           }
         }
-        __syncwarp();                        // vscale is free again
       } else {
         if constexpr (DIRECT) {
-          // 16-bit rows go straight into the operand tile; rows of a page that is not there are zeroed
-          wait_vempty(t);
+          if (!mbar_wait(&vraw[lw], (t / GROUPS) & 1)) ok = false;
+          ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
-          const int c = lane & 15;
-#pragma unroll
-          for (int grp = 0; grp < 2; ++grp) {
-            const int phys = grp ? sh.y : sh.x, off = grp ? sh.z >> 16 : sh.z & 0xffff;
-            const uint8_t* src = vbase + (int64_t)phys * p.v_page_stride + (int64_t)off * p.v_tok_stride + 16 * c;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int r = 2 * i + (lane >> 4), key = 32 * w + 16 * grp + r;
-              uint8_t* at = tile + (c >> 3) * (TILE / 2) + key * 128 + (((c & 7) ^ (key & 7)) << 4);
-              if (phys >= 0) cp_async16(smem_u32(at), src + (int64_t)r * p.v_tok_stride);
-              else *reinterpret_cast<uint4*>(at) = make_uint4(0, 0, 0, 0);
-            }
-          }
-          cp_async_mbar_arrive(&vraw[w]);
-          if (t + 1 < N) convert_k(t + 1);
-          if (!ok || !mbar_wait(&vraw[w], t & 1)) { ok = false; break; }
         } else {
-          if (t + 1 < N) convert_k(t + 1);
-          if (ok) wait_vempty(t);
-          if (!ok) break;
-#pragma unroll 1
-          for (int grp = 0; grp < 2; ++grp) {
-            const uint8_t* src = take();
-            convert_rows<0>(src, tile, 32 * w + 16 * grp);
-            release();
+          cp_async_wait<0>();
+          __syncwarp();
+          if (!wait_empty(vempty, t)) break;
+          convert(vtile, 0);
+          if (more) {
+            settle(t + GROUPS);
+            load_k();
           }
         }
-        // bf16 V becomes fp16 in place: exact for 2^-14 <= |v| < 65520, and P keeps fp16's 11 bits (in bf16 it would keep 8,
-        // which rows of few keys show)
+        // bf16 V becomes fp16 in place: exact for 2^-14 <= |v| < 65520, and P keeps fp16's 11 bits (in bf16 it would
+        // keep 8, which rows of few keys show)
         if (VF == G9_VFMT_BF16 || checked) {
-          __syncwarp();
           const int key = 32 * w + lane;
           const bool dead = lane >= valid;
 #pragma unroll 2
           for (int c = 0; c < 16; ++c) {
-            uint4* at = reinterpret_cast<uint4*>(tile + (c >> 3) * (TILE / 2) + key * 128 + (((c & 7) ^ (key & 7)) << 4));
-            const uint4 x4 = *at;
+            uint4* x = reinterpret_cast<uint4*>(vtile + (c >> 3) * (TILE / 2) + key * 128 + (((c & 7) ^ (key & 7)) << 4));
+            const uint4 x4 = *x;
             uint32_t o[4] = {x4.x, x4.y, x4.z, x4.w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -651,7 +619,7 @@ __global__ void __launch_bounds__(tt::NT, 1) tree_tc_kernel(const __grid_constan
                 o[e] = pack_half2(__uint_as_float(o[e] << 16), __uint_as_float(o[e] & 0xffff0000u));
               if (checked) hit |= clean2(o[e], dead, dead);
             }
-            *at = make_uint4(o[0], o[1], o[2], o[3]);
+            *x = make_uint4(o[0], o[1], o[2], o[3]);
           }
         }
       }
@@ -804,7 +772,7 @@ __global__ void __launch_bounds__(tt::NT, 1) tree_tc_kernel(const __grid_constan
             tmem_ld32(tS + c * 32, x);
             tmem_wait_ld();
             uint32_t v = row_live ? tree_sees(bits, a.words, s.nq, s.ctx, lo, k0 + 32 * c) : 0u;
-            const uint32_t bc = bad >> (8 * c);            // loader warp c holds keys 32c .. 32c + 31
+            const uint32_t bc = bad >> (8 * c);
             if (bc & 1) v &= 0xffff0000u;
             if (bc & 2) v &= 0x0000ffffu;
 #pragma unroll
@@ -818,13 +786,12 @@ __global__ void __launch_bounds__(tt::NT, 1) tree_tc_kernel(const __grid_constan
         // all 128 in registers: the maximum first, then the weights.
         float mx = -INFINITY;
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          uint32_t x[2][32];
-          tmem_ld32(tS + hf * 64, x[0]);
-          tmem_ld32(tS + hf * 64 + 32, x[1]);
+        for (int q4 = 0; q4 < 4; ++q4) {
+          uint32_t x[1][32];
+          tmem_ld32(tS + q4 * 32, x[0]);
           tmem_wait_ld();
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
+          for (int c = 0; c < 1; ++c) {
             float m0 = __uint_as_float(x[c][0]), m1 = __uint_as_float(x[c][1]);
 #pragma unroll
             for (int e = 2; e < 30; e += 4) {
@@ -862,18 +829,16 @@ __global__ void __launch_bounds__(tt::NT, 1) tree_tc_kernel(const __grid_constan
         const uint64_t sc2 = f2pack(sc, sc), nmu2 = f2pack(-mu, -mu);
         uint64_t ls2[2] = {0ull, 0ull};
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          uint32_t x[2][32];
-          tmem_ld32(tS + hf * 64, x[0]);
-          tmem_ld32(tS + hf * 64 + 32, x[1]);
+        for (int q4 = 0; q4 < 4; ++q4) {
+          uint32_t x[32];
+          tmem_ld32(tS + q4 * 32, x);
           tmem_wait_ld();
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
+          for (int c = 0; c < 2; ++c) {
             uint32_t pk[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-              const uint64_t y2 = f2fma(f2pack(__uint_as_float(x[c >> 1][(c & 1) * 16 + 2 * e]),
-                                               __uint_as_float(x[c >> 1][(c & 1) * 16 + 2 * e + 1])), sc2, nmu2);
+              const uint64_t y2 = f2fma(f2pack(__uint_as_float(x[c * 16 + 2 * e]), __uint_as_float(x[c * 16 + 2 * e + 1])), sc2, nmu2);
               float y0, y1;
               f2unpack(y2, y0, y1);
               y0 = fast_exp2(y0);
@@ -881,8 +846,8 @@ __global__ void __launch_bounds__(tt::NT, 1) tree_tc_kernel(const __grid_constan
               ls2[e & 1] = f2add(ls2[e & 1], f2pack(y0, y1));
               pk[e] = pack_half2(y0, y1);
             }
-            // 64 weights take 32 columns: columns whose scores this row has read
-            tmem_st8(tS + hf * 32 + c * 8, pk);
+            // 32 weights take 16 columns: columns whose scores this row has read
+            tmem_st8(tS + q4 * 16 + c * 8, pk);
           }
         }
         float a0, a1, b0, b1;
@@ -1096,7 +1061,7 @@ cudaError_t launch_tree_tc_t(const TreeTcParams& pp, cudaStream_t stream) {
   auto kern = tree_tc_kernel<NQ, VF>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(NQ));
   if (e != cudaSuccess) return e;
-  kern<<<pp.NG * pp.Hkv, NT, smem_bytes(NQ), stream>>>(pp);
+  kern<<<pp.NG * pp.Hkv, threads(NQ), smem_bytes(NQ), stream>>>(pp);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
   if (pp.NG == 1) return cudaSuccess;        // nothing is cut
   const int rows = pp.a.p.seq_q * pp.a.G, groups = (rows + NQ * BM - 1) / (NQ * BM), blocks = pp.rc / 32;
