@@ -258,12 +258,13 @@ __device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, ui
 }
 // 16 raw Q8_0 token rows (PITCH bytes apart, starting 8 * ODD bytes into them)
 // -> rows row0 .. row0 + 15 of an operand tile [row][128] fp16 (two 64-element
-// halves, 128-byte swizzle).  Lane (row, f) converts blocks 2f and 2f + 1: the
-// 68 bytes from 68 f on, read as five aligned 16-byte words.
+// halves, 128-byte swizzle).  Lane (f, row) converts blocks 2f and 2f + 1: the
+// 68 bytes from 68 f on, read as five aligned 16-byte words.  Eight lanes in
+// a run hold eight rows of one half: their stores and loads spread over all banks.
 template <int ODD>
 __device__ __forceinline__ void convert_rows(const uint8_t* raw, uint8_t* tile, int row0) {
-  const int lane = lane_id(), f = lane & 1, row = row0 + (lane >> 1);
-  const uint4* src = reinterpret_cast<const uint4*>(raw + (lane >> 1) * tt::PITCH + 64 * f);
+  const int lane = lane_id(), f = lane >> 4, row = row0 + (lane & 15);
+  const uint4* src = reinterpret_cast<const uint4*>(raw + (lane & 15) * tt::PITCH + 64 * f);
   uint32_t w[20];
 #pragma unroll
   for (int i = 0; i < 5; ++i) {
