@@ -6,13 +6,17 @@
 // Pairs come in groups (one per sequence) and move as if every row of a group
 // were read before any is written, so a path may overlap its destination.  A
 // CTA takes (group, layer, some kv heads), brings the group's rows into shared
-// memory, synchronises and writes them.  Groups must not share slots.
+// memory (every copy in flight at once), synchronises and writes them.  Few
+// groups are spread over more CTAs by giving each fewer heads.  Groups must not
+// share slots.
 //
 // copy_pages: whole pages, for a fork's last partly filled page or a swap.
 //
 // Both move bytes: bound by HBM for many rows, by one launch and two memory
 // round trips for few.  Layer addresses travel as kernel parameters, so a call
 // needs no device-side table.
+#include <type_traits>
+
 #include "common.cuh"
 #include "gfx906_fa_b200.h"
 
@@ -39,25 +43,26 @@ __device__ __forceinline__ void move_bytes(uint8_t* dst, const uint8_t* src) {
   else *reinterpret_cast<uint16_t*>(dst) = *reinterpret_cast<const uint16_t*>(src);
 }
 
-// Rows of `bytes` bytes between the cache (row_at(pair, head)) and `stage`
-// ([pair][head][bytes]); IN: cache to stage.
-template <int W, bool IN, typename RowAt>
-__device__ __forceinline__ void move_rows(uint8_t* stage, int rows, int bytes, RowAt row_at) {
-  const int per_row = bytes / W;
-  for (int i = threadIdx.x; i < rows * per_row; i += kMoveThreads) {
-    const int r = i / per_row, o = (i - r * per_row) * W;
+// Rows of BYTES bytes between the cache (row_at(row)) and `stage`; IN: cache
+// to stage, by asynchronous copies where they are wide enough.
+template <int W, int BYTES, bool IN, typename RowAt>
+__device__ __forceinline__ void move_rows(uint8_t* stage, int rows, RowAt row_at) {
+  constexpr int PER = BYTES / W;
+  for (int i = threadIdx.x; i < rows * PER; i += kMoveThreads) {
+    const int r = i / PER, o = (i - r * PER) * W;
     uint8_t* g = row_at(r);
     if (!g) continue;
-    if (IN) move_bytes<W>(stage + r * bytes + o, g + o);
-    else move_bytes<W>(g + o, stage + r * bytes + o);
+    if (!IN) move_bytes<W>(g + o, stage + r * BYTES + o);
+    else if (W >= 8) cp_async(stage + r * BYTES + o, g + o, W);
+    else move_bytes<W>(stage + r * BYTES + o, g + o);
   }
 }
 
-template <bool IN, typename RowAt>
-__device__ __forceinline__ void move_rows_w(uint8_t* stage, int rows, int bytes, int w, RowAt row_at) {
-  if (w == 16) move_rows<16, IN>(stage, rows, bytes, row_at);
-  else if (w == 8) move_rows<8, IN>(stage, rows, bytes, row_at);
-  else move_rows<2, IN>(stage, rows, bytes, row_at);
+template <int BYTES, bool IN, typename RowAt>
+__device__ __forceinline__ void move_rows_w(uint8_t* stage, int rows, int w, RowAt row_at) {
+  if (w == 16 && BYTES % 16 == 0) move_rows<16, BYTES, IN>(stage, rows, row_at);
+  else if (w >= 8) move_rows<8, BYTES, IN>(stage, rows, row_at);
+  else move_rows<2, BYTES, IN>(stage, rows, row_at);
 }
 
 __global__ void __launch_bounds__(kMoveThreads) move_kv_kernel(const __grid_constant__ MoveArgs a) {
@@ -82,6 +87,7 @@ __global__ void __launch_bounds__(kMoveThreads) move_kv_kernel(const __grid_cons
     at[a.per + i] = skip ? -1 : d;
   }
   __syncthreads();
+  auto at_slot = [&](int p, int which) { return at[which * a.per + p]; };
   auto krow = [&](int r, int which) -> uint8_t* {
     const int p = r / nh, h = h0 + r - p * nh;
     const int64_t s = at[which * a.per + p];
@@ -96,36 +102,62 @@ __global__ void __launch_bounds__(kMoveThreads) move_kv_kernel(const __grid_cons
     const int64_t blk = s / bs;
     return a.v[layer] + blk * a.c.v_page_stride + (s - blk * bs) * a.c.v_tok_stride + h * a.c.v_head_stride;
   };
-  // page-transposed records: a token's scales and values, one element every block_size
+  // Page-transposed records: a token's scales and values, one element every
+  // block_size.  Eight elements a thread in flight.
   auto vrec = [&](bool in) {
-    for (int i = threadIdx.x; i < rows * (D + D / QK); i += kMoveThreads) {
-      const int r = i / (D + D / QK), e = i - r * (D + D / QK);
-      const int p = r / nh, h = h0 + r - p * nh;
-      const int64_t s = at[(in ? 0 : 1) * a.per + p];
-      if (s < 0) continue;
-      const int64_t blk = s / bs;
-      const int off = (int)(s - blk * bs);
-      uint8_t* rec = a.v[layer] + blk * a.c.v_page_stride + h * a.c.v_head_stride;
-      uint8_t* st = vs + r * RB;
-      if (e < D / QK) {
-        uint16_t* g = reinterpret_cast<uint16_t*>(rec + 2 * ((int64_t)e * bs + off));
-        uint16_t* l = reinterpret_cast<uint16_t*>(st) + e;
-        if (in) *l = *g; else *g = *l;
-      } else {
-        const int d = e - D / QK;
-        uint8_t* g = rec + 2 * (D / QK) * bs + (int64_t)d * bs + off;
-        uint8_t* l = st + 2 * (D / QK) + d;
-        if (in) *l = *g; else *g = *l;
+    constexpr int PER = D + D / QK, U = 8;
+    for (int i0 = threadIdx.x; i0 < rows * PER; i0 += kMoveThreads * U) {
+      uint8_t* at[U];
+      uint16_t x[U];
+      int st[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * kMoveThreads;
+        const int r = i / PER, e = i - r * PER;
+        at[u] = nullptr;
+        st[u] = 0;
+        if (i >= rows * PER) continue;
+        const int p = r / nh, h = h0 + r - p * nh;
+        const int64_t s = at_slot(p, in ? 0 : 1);
+        if (s < 0) continue;
+        const int64_t blk = s / bs;
+        const int off = (int)(s - blk * bs);
+        uint8_t* rec = a.v[layer] + blk * a.c.v_page_stride + h * a.c.v_head_stride;
+        // elements 0..3: scales (two bytes), the rest: values
+        at[u] = e < D / QK ? rec + 2 * ((int64_t)e * bs + off) : rec + 2 * (D / QK) * bs + (int64_t)(e - D / QK) * bs + off;
+        st[u] = r * RB + (e < D / QK ? 2 * e : 2 * (D / QK) + e - D / QK) + (e < D / QK ? 1 << 30 : 0);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (!at[u]) continue;
+        const bool wide = st[u] >> 30;
+        const uint8_t* from = in ? at[u] : vs + (st[u] & 0x3fffffff);
+        x[u] = wide ? *reinterpret_cast<const uint16_t*>(from) : *from;
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (!at[u]) continue;
+        const bool wide = st[u] >> 30;
+        uint8_t* to = in ? vs + (st[u] & 0x3fffffff) : at[u];
+        if (wide) *reinterpret_cast<uint16_t*>(to) = x[u];
+        else *to = (uint8_t)x[u];
       }
     }
   };
-  move_rows_w<true>(ks, rows, RB, a.k_w, [&](int r) { return krow(r, 0); });
+  auto vcopy = [&](auto in) {
+    constexpr bool IN = decltype(in)::value;
+    auto row = [&](int r) { return vrow(r, IN ? 0 : 1); };
+    if (a.v_bytes == RB) move_rows_w<RB, IN>(vs, rows, a.v_w, row);
+    else if (a.v_bytes) move_rows_w<2 * D, IN>(vs, rows, a.v_w, row);
+  };
+  move_rows_w<RB, true>(ks, rows, a.k_w, [&](int r) { return krow(r, 0); });
   if (a.c.v_mode == G9_V_Q8T) vrec(true);
-  else if (a.v_bytes) move_rows_w<true>(vs, rows, a.v_bytes, a.v_w, [&](int r) { return vrow(r, 0); });
+  else vcopy(std::true_type());
+  asm volatile("cp.async.wait_all;" ::: "memory");
   __syncthreads();
-  move_rows_w<false>(ks, rows, RB, a.k_w, [&](int r) { return krow(r, 1); });
+  move_rows_w<RB, false>(ks, rows, a.k_w, [&](int r) { return krow(r, 1); });
   if (a.c.v_mode == G9_V_Q8T) vrec(false);
-  else if (a.v_bytes) move_rows_w<false>(vs, rows, a.v_bytes, a.v_w, [&](int r) { return vrow(r, 1); });
+  else vcopy(std::false_type());
 }
 
 // ---------------------------------------------------------------------------
@@ -197,6 +229,11 @@ extern "C" cudaError_t gfx906_fa_move_kv(void* const* k_layers, void* const* v_l
   a.heads = (kMoveSmem - 16 * group_size - 16) / (head_bytes > 0 ? head_bytes : 1);
   if (a.heads < 1) return cudaErrorInvalidValue;
   if (a.heads > c.num_heads_kv) a.heads = c.num_heads_kv;
+  // few groups: halve the heads of a CTA until every SM has four
+  int dev = 0, sms = 148;
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  while (a.heads > 1 && (int64_t)num_groups * num_layers * ((c.num_heads_kv + a.heads - 1) / a.heads) < 4 * (int64_t)sms)
+    a.heads = (a.heads + 1) / 2;
   const int zs = (c.num_heads_kv + a.heads - 1) / a.heads;
   if (zs > 65535) return cudaErrorInvalidValue;
   const int smem = 16 * group_size + ((group_size * a.heads * RB + 15) & ~15) + group_size * a.heads * a.v_bytes;

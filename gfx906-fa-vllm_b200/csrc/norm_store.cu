@@ -33,7 +33,7 @@ struct NormStoreArgs {
   int64_t max_pos;
   const int64_t* slots;
   G9KvCache c;
-  int k_w8, v_w8, v_w16;                           // cache rows: 8-byte (K, Q8_0 V) / 16-byte (16-bit V) aligned
+  int k_w8, v_w8, v_w16, v_rec16;                  // cache rows: 8-byte (K, Q8_0 V), 16-byte (16-bit V), records 16-byte aligned
   int T, Hq, Hkv, rows;                            // rows of a token: Hq + Hkv + (V stored ? Hkv : 0)
   int rpw;                                         // rows of a token a half-warp takes
 };
@@ -44,6 +44,8 @@ constexpr int WARPS = 8;
 constexpr int BATCH = 4;                           // rows in flight per half-warp
 constexpr int RB = D / QK * QBLOCK;
 }  // namespace ns
+
+__device__ __forceinline__ float half_of(uint16_t x) { return __half2float(__ushort_as_half(x)); }
 
 // 8 consecutive elements of a row as loaded; fp32 rows take two registers quads
 struct Raw8 { uint4 a, b; };
@@ -343,68 +345,377 @@ __global__ void __launch_bounds__(ns::WARPS * 32) norm_store_kernel(const __grid
 }
 
 // ---------------------------------------------------------------------------
+// 16-bit tensors of one type on 16-byte rows, 8-byte cache rows: what a model
+// serves.  Queries, keys and values are separate warp items, so that no warp
+// carries another operand's code: a query item is QR rows of a token (their
+// angles loaded once), a key item its kv heads, a value item a run of slots
+// (page-transposed) or a token's heads.
+// ---------------------------------------------------------------------------
+struct FastItems {
+  int qr, pq, pk, pv;            // query rows an item; items a token of queries, keys and (rows) values
+  int64_t nq, nk, nv;            // items
+};
+
+// The tokens of a value item.  Page-transposed V is written by runs: tokens
+// whose slots follow one another inside an aligned group of 16, at most 16.  A
+// warp looks at 16 tokens and takes the runs that start among them; a run of
+// all 16 slots leaves as 16-byte stores (one per dim), where single tokens cost
+// a byte store per element.  Returns a bit per token i = 0..31 that continues the run of token i - 1.
+__device__ __forceinline__ uint32_t run_bits(const int64_t* slots, int t0, int T, int64_t end, int64_t& mine) {
+  const int t = t0 + lane_id();
+  mine = t < T ? slots[t] : -1;
+  const int64_t before = t > 0 && t <= T ? slots[t - 1] : -1;
+  const bool ok = mine >= 0 && mine < end;
+  if (mine >= end) raise_error(ERR_BAD_INDEX);
+  if (!ok) mine = -1;
+  return __ballot_sync(0xffffffffu, ok && before >= 0 && mine == before + 1 && (mine & 15) != 0);
+}
+
+template <int DT>
+__device__ __forceinline__ void widen16(uint4 r, float v[8]) {
+  Raw8 x;
+  x.a = r;
+  widen8(x, DT, v);
+}
+
+// 4 x 4 bytes: word i of w holds byte i of each result word
+__device__ __forceinline__ void transpose4(uint32_t w[4]) {
+  const uint32_t a = __byte_perm(w[0], w[1], 0x5140), b = __byte_perm(w[2], w[3], 0x5140);
+  const uint32_t c = __byte_perm(w[0], w[1], 0x7362), d = __byte_perm(w[2], w[3], 0x7362);
+  w[0] = __byte_perm(a, b, 0x5410);
+  w[1] = __byte_perm(a, b, 0x7632);
+  w[2] = __byte_perm(c, d, 0x5410);
+  w[3] = __byte_perm(c, d, 0x7632);
+}
+
+template <int DT>
+__device__ __forceinline__ void norm_rope_row(const NormStoreArgs& a, const Angles& g, const float w[8], bool norm, int hl, float v[8]) {
+  if (norm) norm8(v, w, a.eps);
+  rotate8(a, g, hl, v);
+}
+
+template <int DT>
+__global__ void __launch_bounds__(ns::WARPS * 32) norm_store_fast_kernel(const __grid_constant__ NormStoreArgs a,
+                                                                         const __grid_constant__ FastItems f) {
+  using namespace ns;
+  __shared__ __align__(16) uint8_t stage_all[WARPS][16 * 128 + 128];
+  uint8_t* stage = stage_all[warp_id()];
+  const int lane = lane_id(), hl = lane & 15, half = lane >> 4;
+  const int64_t total = f.nq + f.nk + f.nv;
+  for (int64_t it = (int64_t)blockIdx.x * WARPS + warp_id(); it < total; it += (int64_t)gridDim.x * WARPS) {
+    if (it < f.nq + f.nk) {
+      const bool isq = it < f.nq;
+      const int64_t i = isq ? it : it - f.nq;
+      const int parts = isq ? f.pq : f.pk;
+      const int t = (int)(i / parts), H = isq ? a.Hq : a.Hkv;
+      const int per = isq ? f.qr : 8;                    // rows of this item: per / 2 a half-warp
+      const int r0 = (int)(i - (int64_t)t * parts) * per;
+      const int rows = min(per, H - r0);
+      int64_t pos = a.positions[t];
+      if (pos < 0 || pos >= a.max_pos) {
+        raise_error(ERR_BAD_INDEX);
+        pos = 0;
+      }
+      const uint16_t* src = reinterpret_cast<const uint16_t*>(isq ? a.q : a.k) + (int64_t)t * (isq ? a.q_tok : a.k_tok) + 8 * hl;
+      const int64_t hs = isq ? a.q_head : a.k_head;
+      uint4 raw[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) raw[x] = *reinterpret_cast<const uint4*>(src + (int64_t)(r0 + min(2 * x + half, rows - 1)) * hs);
+      Angles g;
+      load_angles(a, pos, hl, g);
+      const void* wp = isq ? a.q_w : a.k_w;
+      float w[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      if (wp) widen8(load_raw8(wp, 8 * hl, isq ? a.qw_dt : a.kw_dt, false), isq ? a.qw_dt : a.kw_dt, w);
+      if (isq) {
+        uint16_t* dst = reinterpret_cast<uint16_t*>(a.q_out) + (int64_t)t * a.qo_tok + 8 * hl;
+        for (int b = 0; b < rows; b += 8) {
+          uint4 cur[4];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) cur[x] = raw[x];
+          if (b + 8 < rows) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x) raw[x] = *reinterpret_cast<const uint4*>(src + (int64_t)(r0 + min(b + 8 + 2 * x + half, rows - 1)) * hs);
+          }
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            if (b + 2 * x >= rows) break;                // the same for both halves
+            float v[8];
+            widen16<DT>(cur[x], v);
+            norm_rope_row<DT>(a, g, w, wp != nullptr, hl, v);
+            const uint4 packed = round8(v, DT);
+            const int r = b + 2 * x + half;
+            if (r < rows) *reinterpret_cast<uint4*>(dst + (int64_t)(r0 + r) * a.qo_head) = packed;
+          }
+        }
+      } else {
+        const int64_t slot = a.slots[t];
+        const int64_t blk = slot / a.c.block_size;
+        const int off = (int)(slot - blk * a.c.block_size);
+        bool stored = slot >= 0;
+        if (stored && a.c.num_blocks > 0 && blk >= a.c.num_blocks) {
+          raise_error(ERR_BAD_INDEX);
+          stored = false;
+        }
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          if (2 * x >= rows) break;
+          const int r = 2 * x + half;
+          float v[8];
+          widen16<DT>(raw[x], v);
+          norm_rope_row<DT>(a, g, w, wp != nullptr, hl, v);
+          const uint4 packed = round8(v, DT);
+          if (a.k_out && r < rows)
+            *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.k_out) + (int64_t)t * a.ko_tok + (int64_t)(r0 + r) * a.ko_head + 8 * hl) = packed;
+          if (!stored) continue;                         // the same for the warp
+          uint16_t scale;
+          const uint2 q = quant8(v, scale);
+          uint8_t* dst = a.c.k + blk * a.c.k_page_stride + off * a.c.k_tok_stride + (int64_t)(r0 + r) * a.c.k_head_stride;
+          write_q8_row(dst, q, scale, hl, r < rows, true, stage + half * RB);
+        }
+      }
+      continue;
+    }
+    const int64_t i = it - f.nq - f.nk;
+    if (a.c.v_mode != G9_V_Q8T) {
+      // token rows: eight kv heads of a token
+      const int t = (int)(i / f.pv), r0 = (int)(i - (int64_t)t * f.pv) * 8, rows = min(8, a.Hkv - r0);
+      const uint16_t* src = reinterpret_cast<const uint16_t*>(a.v) + (int64_t)t * a.v_tok + 8 * hl;
+      uint4 raw[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) raw[x] = *reinterpret_cast<const uint4*>(src + (int64_t)(r0 + min(2 * x + half, rows - 1)) * a.v_head);
+      const int64_t slot = a.slots[t];
+      const int64_t blk = slot / a.c.block_size;
+      const int off = (int)(slot - blk * a.c.block_size);
+      if (slot < 0) continue;
+      if (a.c.num_blocks > 0 && blk >= a.c.num_blocks) {
+        raise_error(ERR_BAD_INDEX);
+        continue;
+      }
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        if (2 * x >= rows) break;
+        const int r = 2 * x + half;
+        uint8_t* dst = a.c.v + blk * a.c.v_page_stride + off * a.c.v_tok_stride + (int64_t)(r0 + r) * a.c.v_head_stride;
+        if (a.c.v_mode == G9_V_COPY16) {
+          if (r < rows) *reinterpret_cast<uint4*>(dst + 16 * hl) = raw[x];
+        } else {
+          float v[8];
+          widen16<DT>(raw[x], v);
+          uint16_t scale;
+          const uint2 q = quant8(v, scale);
+          write_q8_row(dst, q, scale, hl, r < rows, true, stage + half * RB);
+        }
+      }
+      continue;
+    }
+    // ---- page-transposed V: (16 tokens, kv head) ----------------------------------
+    const int h = (int)(i % a.Hkv);
+    const int t0 = (int)(i / a.Hkv) * 16;
+    const int bs = a.c.block_size;
+    int64_t mine;
+    const uint32_t cont = run_bits(a.slots, t0, a.T, a.c.num_blocks > 0 ? (int64_t)a.c.num_blocks * bs : INT64_MAX, mine);
+    const uint32_t live = __ballot_sync(0xffffffffu, mine >= 0);
+    for (uint32_t heads = live & ~cont & 0xffffu; heads; heads &= heads - 1) {
+      const int i0 = __ffs(heads) - 1;                   // the run's first token
+      const int n = 1 + (i0 == 31 ? 0 : __ffs(~(cont >> (i0 + 1))) - 1);         // cont has a zero above bit 31 - i0
+      const int64_t slot = __shfl_sync(0xffffffffu, mine, i0);
+      const int64_t blk = slot / bs;
+      const int off = (int)(slot - blk * bs), sub = off & 15;
+      const uint16_t* src = reinterpret_cast<const uint16_t*>(a.v) + (int64_t)(t0 + i0) * a.v_tok + (int64_t)h * a.v_head + 8 * hl;
+      uint16_t* scales = reinterpret_cast<uint16_t*>(stage + 16 * 128);          // [block][16]
+      // quantised rows into [slot % 16][dim], two tokens a step, four steps' loads in flight
+      for (int b = 0; b < n; b += 8) {
+        uint4 raw[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) raw[x] = *reinterpret_cast<const uint4*>(src + (int64_t)min(b + 2 * x + half, n - 1) * a.v_tok);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          if (b + 2 * x >= n) break;
+          const int k = b + 2 * x + half;
+          float v[8];
+          widen16<DT>(raw[x], v);
+          uint16_t scale;
+          const uint2 q = quant8(v, scale);
+          if (k < n) {
+            *reinterpret_cast<uint2*>(stage + (sub + k) * 128 + 8 * hl) = q;
+            if ((hl & 3) == 0) scales[(hl >> 2) * 16 + sub + k] = scale;
+          }
+        }
+      }
+      __syncwarp();
+      uint8_t* rec = a.c.v + blk * a.c.v_page_stride + (int64_t)h * a.c.v_head_stride;
+      uint8_t* sdst = rec + 2 * (off - sub);
+      uint8_t* vdst = rec + 2 * (D / QK) * bs + (off - sub);
+      // lane: dims 4 * lane .. + 3, 16 tokens each
+      uint32_t y[4][4];
+#pragma unroll
+      for (int k4 = 0; k4 < 4; ++k4) {
+        uint32_t x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = *reinterpret_cast<const uint32_t*>(stage + (4 * k4 + e) * 128 + 4 * lane);
+        transpose4(x);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e][k4] = x[e];
+      }
+      if (n == 16 && a.v_rec16) {
+        if (lane < 8) *reinterpret_cast<uint4*>(sdst + 2 * (lane >> 1) * bs + 16 * (lane & 1)) =
+            *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(scales) + 16 * lane);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          *reinterpret_cast<uint4*>(vdst + (int64_t)(4 * lane + e) * bs) = make_uint4(y[e][0], y[e][1], y[e][2], y[e][3]);
+      } else {
+        for (int x = lane; x < 4 * n; x += 32) {
+          const int blkq = x / n, k = sub + x - blkq * n;
+          *reinterpret_cast<uint16_t*>(sdst + 2 * (blkq * bs + k)) = scales[blkq * 16 + k];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int k = 0; k < 16; ++k)
+            if (k >= sub && k < sub + n) vdst[(int64_t)(4 * lane + e) * bs + k] = (uint8_t)(y[e][k >> 2] >> (8 * (k & 3)));
+      }
+      __syncwarp();
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
 // read_kv: rows of the cache by slot, as 16- or 32-bit values
 // ---------------------------------------------------------------------------
 struct ReadArgs {
   G9KvCache c;
   const int64_t* slots;
   int N, Hkv, out_dt, v_src;                       // v_src: DT_F16 / DT_BF16 of 16-bit V rows
+  int k_w8, v_w8, v_w16, v_rec16;                  // rows on 8- and 16-byte boundaries, records on 16
+  int64_t nrows;                                   // row items (two rows a warp); run items follow
+  int64_t nruns;
   void* k_out; void* v_out;                        // [N, Hkv, 128]; v_out may be null
 };
 
-__device__ __forceinline__ void q8_lane(const uint8_t* row, int hl, float v[8]) {
-  const uint8_t* b = row + (hl >> 2) * QBLOCK;
-  const float d = __half2float(__ushort_as_half(*reinterpret_cast<const uint16_t*>(b)));
-  const uint16_t* q = reinterpret_cast<const uint16_t*>(b + 2 + 8 * (hl & 3));
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const uint16_t w = q[e];
-    v[2 * e] = (float)(int8_t)(w & 0xff) * d;
-    v[2 * e + 1] = (float)(int8_t)(w >> 8) * d;
+// elements 8 * hl .. + 7 of a Q8_0 row
+__device__ __forceinline__ void q8_lane(const uint8_t* row, int hl, bool w8, float v[8]) {
+  const int blk = hl >> 2, o = blk * QBLOCK + 2 + 8 * (hl & 3);
+  uint64_t x;
+  float d;
+  if (w8) {
+    // the 8 values start 2, 4, 6 or 0 bytes into an aligned word: two words and a shift
+    const uint64_t* p = reinterpret_cast<const uint64_t*>(row + (o & ~7));
+    const int sh = (o & 7) * 8;
+    const uint64_t lo = p[0], hi = sh ? p[1] : 0;
+    x = sh ? lo >> sh | hi << (64 - sh) : lo;
+    d = half_of(*reinterpret_cast<const uint16_t*>(row + blk * QBLOCK));
+  } else {
+    const uint16_t* q = reinterpret_cast<const uint16_t*>(row + o);
+    x = (uint64_t)q[0] | (uint64_t)q[1] << 16 | (uint64_t)q[2] << 32 | (uint64_t)q[3] << 48;
+    d = half_of(*reinterpret_cast<const uint16_t*>(row + blk * QBLOCK));
   }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = (float)(int8_t)(x >> (8 * e)) * d;
 }
 
+// Row items: half a warp reads one K or V row.  Run items: page-transposed V by
+// runs of slots (run_bits): a lane takes 4 dims x 16 tokens as four 16-byte
+// loads, whatever part of the 16 the run covers.
 __global__ void __launch_bounds__(ns::WARPS * 32) read_kv_kernel(const __grid_constant__ ReadArgs a) {
   using namespace ns;
-  const int hl = threadIdx.x & 15;
-  const int64_t rows = (int64_t)a.N * a.Hkv;
-  const int64_t step = (int64_t)gridDim.x * WARPS * 2;
-  for (int64_t r = (int64_t)blockIdx.x * WARPS * 2 + (threadIdx.x >> 4); r < rows; r += step) {
-    const int64_t n = r / a.Hkv;
-    const int h = (int)(r - n * a.Hkv);
-    const int64_t slot = a.slots[n];
-    float k[8], v[8];
+  const int lane = lane_id(), hl = lane & 15;
+  const int bs = a.c.block_size;
+  const int64_t end = a.c.num_blocks > 0 ? (int64_t)a.c.num_blocks * bs : INT64_MAX;
+  const int64_t total = a.nrows + a.nruns, krows = (int64_t)a.N * a.Hkv;
+  for (int64_t it = (int64_t)blockIdx.x * WARPS + warp_id(); it < total; it += (int64_t)gridDim.x * WARPS) {
+    if (it < a.nrows) {
+      const int64_t y = 2 * it + (lane >> 4);
+      const bool isv = y >= krows;
+      const int64_t r = isv ? y - krows : y;
+      if (r >= krows) continue;
+      const int64_t n = r / a.Hkv;
+      const int h = (int)(r - n * a.Hkv);
+      const int64_t slot = a.slots[n];
+      float v[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) k[e] = v[e] = 0.f;
-    const int64_t blk = slot / a.c.block_size;
-    const int off = (int)(slot - blk * a.c.block_size);
-    const bool bad = slot >= 0 && a.c.num_blocks > 0 && blk >= a.c.num_blocks;
-    if (bad) raise_error(ERR_BAD_INDEX);
-    if (slot >= 0 && !bad) {
-      q8_lane(a.c.k + blk * a.c.k_page_stride + off * a.c.k_tok_stride + h * a.c.k_head_stride, hl, k);
-      if (a.v_out) {
-        if (a.c.v_mode == G9_V_Q8T) {
+      for (int e = 0; e < 8; ++e) v[e] = 0.f;
+      if (slot >= end) raise_error(ERR_BAD_INDEX);
+      if (slot >= 0 && slot < end) {
+        const int64_t blk = slot / bs;
+        const int off = (int)(slot - blk * bs);
+        if (!isv) {
+          q8_lane(a.c.k + blk * a.c.k_page_stride + off * a.c.k_tok_stride + h * a.c.k_head_stride, hl, a.k_w8, v);
+        } else if (a.c.v_mode == G9_V_Q8T) {             // records off 16-byte boundaries
           const uint8_t* rec = a.c.v + blk * a.c.v_page_stride + h * a.c.v_head_stride;
-          const int bs = a.c.block_size;
-          const float d = __half2float(__ushort_as_half(
-              *reinterpret_cast<const uint16_t*>(rec + 2 * ((int64_t)(hl >> 2) * bs + off))));
+          const float d = half_of(*reinterpret_cast<const uint16_t*>(rec + 2 * ((int64_t)(hl >> 2) * bs + off)));
           const int8_t* q = reinterpret_cast<const int8_t*>(rec + 2 * (D / QK) * bs + (int64_t)8 * hl * bs + off);
 #pragma unroll
           for (int e = 0; e < 8; ++e) v[e] = (float)q[(int64_t)e * bs] * d;
         } else {
           const uint8_t* row = a.c.v + blk * a.c.v_page_stride + off * a.c.v_tok_stride + h * a.c.v_head_stride;
-          if (a.c.v_mode == G9_V_Q8) q8_lane(row, hl, v);
-          else
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = load_one(row, 8 * hl + e, a.v_src);
+          if (a.c.v_mode == G9_V_Q8) q8_lane(row, hl, a.v_w8, v);
+          else widen8(load_raw8(row, 8 * hl, a.v_src, a.v_w16), a.v_src, v);
         }
       }
+      const uint4 packed = round8(v, a.out_dt);
+      store8(isv ? a.v_out : a.k_out, r * D + 8 * hl, a.out_dt, true, v, packed);
+      continue;
     }
-    const uint4 pk = round8(k, a.out_dt);
-    store8(a.k_out, r * D + 8 * hl, a.out_dt, true, k, pk);
-    if (a.v_out) {
-      const uint4 pv = round8(v, a.out_dt);
-      store8(a.v_out, r * D + 8 * hl, a.out_dt, true, v, pv);
+    const int64_t i = it - a.nrows;
+    const int h = (int)(i % a.Hkv);
+    const int t0 = (int)(i / a.Hkv) * 16;
+    int64_t mine;
+    const uint32_t cont = run_bits(a.slots, t0, a.N, end, mine);
+    const uint32_t live = __ballot_sync(0xffffffffu, mine >= 0);
+    for (uint32_t heads = ~(live & cont) & 0xffffu; heads; heads &= heads - 1) {
+      const int i0 = __ffs(heads) - 1;
+      if (t0 + i0 >= a.N) break;
+      const int n = 1 + __ffs(~(cont >> (i0 + 1))) - 1;
+      const int64_t slot = __shfl_sync(0xffffffffu, mine, i0);
+      uint4 q[4];
+      uint4 s[2];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) q[e] = make_uint4(0, 0, 0, 0);
+      s[0] = s[1] = make_uint4(0, 0, 0, 0);
+      int sub = 0;
+      if (slot >= 0) {
+        const int64_t blk = slot / bs;
+        const int off = (int)(slot - blk * bs);
+        sub = off & 15;
+        const uint8_t* rec = a.c.v + blk * a.c.v_page_stride + (int64_t)h * a.c.v_head_stride;
+        const uint4* sp = reinterpret_cast<const uint4*>(rec + 2 * ((int64_t)(lane >> 3) * bs + off - sub));
+        s[0] = sp[0];
+        s[1] = sp[1];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          q[e] = *reinterpret_cast<const uint4*>(rec + 2 * (D / QK) * bs + (int64_t)(4 * lane + e) * bs + off - sub);
+      }
+      const uint32_t sw[8] = {s[0].x, s[0].y, s[0].z, s[0].w, s[1].x, s[1].y, s[1].z, s[1].w};
+#pragma unroll
+      for (int k4 = 0; k4 < 4; ++k4) {
+        uint32_t x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = k4 == 0 ? q[e].x : k4 == 1 ? q[e].y : k4 == 2 ? q[e].z : q[e].w;
+        transpose4(x);                                   // x[k]: token 4 * k4 + k, this lane's 4 dims
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int tok = 4 * k4 + k;
+          if (tok < sub || tok >= sub + n) continue;
+          const float d = half_of((uint16_t)(sw[tok >> 1] >> (16 * (tok & 1))));
+          float v[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = (float)(int8_t)(x[k] >> (8 * e)) * d;
+          const int64_t at = ((int64_t)(t0 + i0 + tok - sub) * a.Hkv + h) * D + 4 * lane;
+          if (a.out_dt == DT_F32) {
+            *reinterpret_cast<float4*>(reinterpret_cast<float*>(a.v_out) + at) = make_float4(v[0], v[1], v[2], v[3]);
+          } else {
+            uint2 o;
+            if (a.out_dt == DT_F16) {
+              const __half2 x0 = __floats2half2_rn(v[0], v[1]), x1 = __floats2half2_rn(v[2], v[3]);
+              o = make_uint2(*reinterpret_cast<const uint32_t*>(&x0), *reinterpret_cast<const uint32_t*>(&x1));
+            } else {
+              const __nv_bfloat162 x0 = __floats2bfloat162_rn(v[0], v[1]), x1 = __floats2bfloat162_rn(v[2], v[3]);
+              o = make_uint2(*reinterpret_cast<const uint32_t*>(&x0), *reinterpret_cast<const uint32_t*>(&x1));
+            }
+            *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.v_out) + at) = o;
+          }
+        }
+      }
     }
   }
 }
@@ -479,8 +790,31 @@ extern "C" cudaError_t gfx906_fa_norm_rope_store_kv(
   a.v_w16 = aligned((uintptr_t)cache->v, cache->v_page_stride, cache->v_tok_stride, cache->v_head_stride, 16);
   a.T = num_tokens; a.Hq = query ? num_heads_q : 0; a.Hkv = cache->num_heads_kv;
   a.rows = a.Hq + a.Hkv + (cache->v_mode != G9_V_NONE ? a.Hkv : 0);
+  a.v_rec16 = cache->block_size % 16 == 0 &&
+              aligned((uintptr_t)cache->v, cache->v_page_stride, cache->v_head_stride, 0, 16);
   const int sms = ns_sms();
-  // few tokens: a half-warp a row, so that every SM has work; many: BATCH rows share a token's angles and loads overlap
+  const bool withv = cache->v_mode != G9_V_NONE;
+  const bool fast = key_dtype != G9_DT_F32 && (!query || query_dtype == key_dtype) && (!withv || value_dtype == key_dtype) &&
+                    a.k_vec && (!query || (a.q_vec && a.qo_vec)) && (!key_out || a.ko_vec) && (!withv || a.v_vec) && a.k_w8 &&
+                    (cache->v_mode != G9_V_Q8 || a.v_w8) && (cache->v_mode != G9_V_COPY16 || a.v_w16) &&
+                    (cache->v_mode != G9_V_Q8T || cache->block_size % 16 == 0);
+  if (fast) {
+    FastItems f{};
+    // few tokens: 8 query rows a warp, so that more SMs have work; many: 16, which share the token's angles and weights
+    f.qr = (int64_t)num_tokens * a.Hq < (int64_t)sms * ns::WARPS * 32 ? 8 : 16;
+    f.pq = (a.Hq + f.qr - 1) / f.qr;
+    f.pk = (a.Hkv + 7) / 8;
+    f.pv = (a.Hkv + 7) / 8;
+    f.nq = (int64_t)num_tokens * f.pq;
+    f.nk = (int64_t)num_tokens * f.pk;
+    f.nv = !withv ? 0 : cache->v_mode == G9_V_Q8T ? (int64_t)((num_tokens + 15) / 16) * a.Hkv : (int64_t)num_tokens * f.pv;
+    const int64_t want = (f.nq + f.nk + f.nv + ns::WARPS - 1) / ns::WARPS, cap = (int64_t)sms * 32;
+    const int grid = (int)(want < cap ? want : cap);
+    if (key_dtype == G9_DT_F16) norm_store_fast_kernel<DT_F16><<<grid, ns::WARPS * 32, 0, stream>>>(a, f);
+    else norm_store_fast_kernel<DT_BF16><<<grid, ns::WARPS * 32, 0, stream>>>(a, f);
+    return cudaGetLastError();
+  }
+  // other types, alignments and page sizes; a half-warp a row when rows are few, else BATCH rows share a token's angles
   a.rpw = (int64_t)num_tokens * a.rows < (int64_t)sms * ns::WARPS * 2 * ns::BATCH ? 1 : ns::BATCH;
   const int64_t items = (int64_t)num_tokens * ((a.rows + a.rpw - 1) / a.rpw);
   const int64_t want = (items + ns::WARPS * 2 - 1) / (ns::WARPS * 2);
@@ -496,9 +830,19 @@ extern "C" cudaError_t gfx906_fa_read_kv(const G9KvCache* cache, int value_dtype
   if (value_out && cache->v_mode == G9_V_NONE) return cudaErrorInvalidValue;
   if (value_out && cache->v_mode == G9_V_COPY16 && value_dtype != G9_DT_F16 && value_dtype != G9_DT_BF16)
     return cudaErrorInvalidValue;
-  ReadArgs a{*cache, slots, num_rows, cache->num_heads_kv, out_dtype, value_dtype, key_out, value_out};
-  const int64_t want = ((int64_t)num_rows * a.Hkv + ns::WARPS * 2 - 1) / (ns::WARPS * 2);
-  const int64_t cap = (int64_t)ns_sms() * 32;
+  ReadArgs a{};
+  a.c = *cache;
+  a.slots = slots; a.N = num_rows; a.Hkv = cache->num_heads_kv; a.out_dt = out_dtype; a.v_src = value_dtype;
+  a.k_out = key_out; a.v_out = value_out;
+  a.k_w8 = aligned((uintptr_t)cache->k, cache->k_page_stride, cache->k_tok_stride, cache->k_head_stride, 8);
+  a.v_w8 = aligned((uintptr_t)cache->v, cache->v_page_stride, cache->v_tok_stride, cache->v_head_stride, 8);
+  a.v_w16 = aligned((uintptr_t)cache->v, cache->v_page_stride, cache->v_tok_stride, cache->v_head_stride, 16);
+  a.v_rec16 = cache->block_size % 16 == 0 && aligned((uintptr_t)cache->v, cache->v_page_stride, cache->v_head_stride, 0, 16);
+  const int64_t rows = (int64_t)num_rows * a.Hkv;
+  const bool runs = value_out && cache->v_mode == G9_V_Q8T && a.v_rec16;
+  a.nrows = (rows * (value_out && !runs ? 2 : 1) + 1) / 2;
+  a.nruns = runs ? (int64_t)((num_rows + 15) / 16) * a.Hkv : 0;
+  const int64_t want = (a.nrows + a.nruns + ns::WARPS - 1) / ns::WARPS, cap = (int64_t)ns_sms() * 32;
   read_kv_kernel<<<(int)(want < cap ? want : cap), ns::WARPS * 32, 0, stream>>>(a);
   return cudaGetLastError();
 }
