@@ -72,35 +72,31 @@ __global__ void __launch_bounds__(kMoveThreads) move_kv_kernel(const __grid_cons
   const int rows = a.per * nh;
   constexpr int D = 128, RB = D / QK * QBLOCK;
   const int bs = a.c.block_size;
-  int64_t* at = reinterpret_cast<int64_t*>(smem);  // [per] source slot, [per] destination slot; -1: skip
+  // [source / destination][pair]: page and offset (page -1: skip the pair)
+  int2* slot = reinterpret_cast<int2*>(smem);
   uint8_t* ks = smem + 16 * a.per;
   uint8_t* vs = ks + ((a.per * a.heads * RB + 15) & ~15);
   for (int i = threadIdx.x; i < a.per; i += kMoveThreads) {
-    int64_t s = a.src[(int64_t)blockIdx.x * a.per + i], d = a.dst[(int64_t)blockIdx.x * a.per + i];
+    const int64_t s = a.src[(int64_t)blockIdx.x * a.per + i], d = a.dst[(int64_t)blockIdx.x * a.per + i];
     bool skip = s < 0 || d < 0 || s == d;
     const int64_t end = (int64_t)a.c.num_blocks * bs;
     if (!skip && (s >= end || d >= end)) {
       raise_error(ERR_BAD_INDEX);
       skip = true;
     }
-    at[i] = skip ? -1 : s;
-    at[a.per + i] = skip ? -1 : d;
+    slot[i] = skip ? make_int2(-1, 0) : make_int2((int)(s / bs), (int)(s % bs));
+    slot[a.per + i] = skip ? make_int2(-1, 0) : make_int2((int)(d / bs), (int)(d % bs));
   }
   __syncthreads();
-  auto at_slot = [&](int p, int which) { return at[which * a.per + p]; };
   auto krow = [&](int r, int which) -> uint8_t* {
     const int p = r / nh, h = h0 + r - p * nh;
-    const int64_t s = at[which * a.per + p];
-    if (s < 0) return nullptr;
-    const int64_t blk = s / bs;
-    return a.k[layer] + blk * a.c.k_page_stride + (s - blk * bs) * a.c.k_tok_stride + h * a.c.k_head_stride;
+    const int2 s = slot[which * a.per + p];
+    return s.x < 0 ? nullptr : a.k[layer] + s.x * a.c.k_page_stride + s.y * a.c.k_tok_stride + h * a.c.k_head_stride;
   };
   auto vrow = [&](int r, int which) -> uint8_t* {
     const int p = r / nh, h = h0 + r - p * nh;
-    const int64_t s = at[which * a.per + p];
-    if (s < 0) return nullptr;
-    const int64_t blk = s / bs;
-    return a.v[layer] + blk * a.c.v_page_stride + (s - blk * bs) * a.c.v_tok_stride + h * a.c.v_head_stride;
+    const int2 s = slot[which * a.per + p];
+    return s.x < 0 ? nullptr : a.v[layer] + s.x * a.c.v_page_stride + s.y * a.c.v_tok_stride + h * a.c.v_head_stride;
   };
   // Page-transposed records: a token's scales and values, one element every
   // block_size.  Eight elements a thread in flight.
@@ -118,11 +114,10 @@ __global__ void __launch_bounds__(kMoveThreads) move_kv_kernel(const __grid_cons
         st[u] = 0;
         if (i >= rows * PER) continue;
         const int p = r / nh, h = h0 + r - p * nh;
-        const int64_t s = at_slot(p, in ? 0 : 1);
-        if (s < 0) continue;
-        const int64_t blk = s / bs;
-        const int off = (int)(s - blk * bs);
-        uint8_t* rec = a.v[layer] + blk * a.c.v_page_stride + h * a.c.v_head_stride;
+        const int2 s = slot[(in ? 0 : a.per) + p];
+        if (s.x < 0) continue;
+        const int off = s.y;
+        uint8_t* rec = a.v[layer] + s.x * a.c.v_page_stride + h * a.c.v_head_stride;
         // elements 0..3: scales (two bytes), the rest: values
         at[u] = e < D / QK ? rec + 2 * ((int64_t)e * bs + off) : rec + 2 * (D / QK) * bs + (int64_t)(e - D / QK) * bs + off;
         st[u] = r * RB + (e < D / QK ? 2 * e : 2 * (D / QK) + e - D / QK) + (e < D / QK ? 1 << 30 : 0);

@@ -14,6 +14,7 @@
 // three times.
 #include "common.cuh"
 #include "gfx906_fa_b200.h"
+#include "tcgen05.cuh"
 
 namespace g9 {
 
@@ -33,6 +34,7 @@ struct NormStoreArgs {
   int64_t max_pos;
   const int64_t* slots;
   G9KvCache c;
+  int bs_log2;                                     // of the page size, -1: not a power of two
   int k_w8, v_w8, v_w16, v_rec16;                  // cache rows: 8-byte (K, Q8_0 V), 16-byte (16-bit V), records 16-byte aligned
   int T, Hq, Hkv, rows;                            // rows of a token: Hq + Hkv + (V stored ? Hkv : 0)
   int rpw;                                         // rows of a token a half-warp takes
@@ -46,6 +48,9 @@ constexpr int RB = D / QK * QBLOCK;
 }  // namespace ns
 
 __device__ __forceinline__ float half_of(uint16_t x) { return __half2float(__ushort_as_half(x)); }
+
+// page of a slot; a power-of-two page size spares the 64-bit division (log2 < 0: it is none)
+__device__ __forceinline__ int64_t slot_page(int64_t slot, int bs, int log2) { return log2 >= 0 ? slot >> log2 : slot / bs; }
 
 // 8 consecutive elements of a row as loaded; fp32 rows take two registers quads
 struct Raw8 { uint4 a, b; };
@@ -165,7 +170,7 @@ __device__ __forceinline__ uint2 quant8(const float v[8], uint16_t& scale) {
 
 // cos / sin of this lane's 8 elements.  NeoX: element e pairs with e +- rot/2;
 // otherwise 2j with 2j + 1, four pairs a lane.
-struct Angles { float c[8], s[8]; };
+struct Angles { float c[8] = {}, s[8] = {}; };
 
 __device__ __forceinline__ void load_angles(const NormStoreArgs& a, int64_t pos, int hl, Angles& g) {
   const int half = a.rot >> 1, e0 = 8 * hl;
@@ -261,7 +266,7 @@ __global__ void __launch_bounds__(ns::WARPS * 32) norm_store_kernel(const __grid
       raise_error(ERR_BAD_INDEX);
       pos = 0;
     }
-    int64_t blk = slot / a.c.block_size;
+    const int64_t blk = slot_page(slot, a.c.block_size, a.bs_log2);
     const int off = (int)(slot - blk * a.c.block_size);
     bool stored = on && slot >= 0;
     if (stored && a.c.num_blocks > 0 && blk >= a.c.num_blocks) {
@@ -353,7 +358,7 @@ __global__ void __launch_bounds__(ns::WARPS * 32) norm_store_kernel(const __grid
 // ---------------------------------------------------------------------------
 struct FastItems {
   int qr, pq, pk, pv;            // query rows an item; items a token of queries, keys and (rows) values
-  int64_t nq, nk, nv;            // items
+  uint32_t nq, nk, nv;           // items, below 2^31 in all
 };
 
 // The tokens of a value item.  Page-transposed V is written by runs: tokens
@@ -388,28 +393,75 @@ __device__ __forceinline__ void transpose4(uint32_t w[4]) {
   w[3] = __byte_perm(c, d, 0x7632);
 }
 
-template <int DT>
-__device__ __forceinline__ void norm_rope_row(const NormStoreArgs& a, const Angles& g, const float w[8], bool norm, int hl, float v[8]) {
-  if (norm) norm8(v, w, a.eps);
-  rotate8(a, g, hl, v);
+// A half-warp's angles and weight as packed pairs of fp32 (f32x2 arithmetic: one
+// instruction, two elements).  s carries the sign of its term; lanes past the rotated part keep their values.
+struct Pairs { uint64_t c[4], s[4], w[4]; };
+
+__device__ __forceinline__ void make_pairs(const NormStoreArgs& a, const Angles& g, const float w[8], int hl, Pairs& o) {
+  const bool lower = hl < (a.rot >> 4);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    o.w[e] = f2pack(w[2 * e], w[2 * e + 1]);
+    if (a.neox) {
+      o.c[e] = f2pack(g.c[2 * e], g.c[2 * e + 1]);
+      o.s[e] = lower ? f2pack(-g.s[2 * e], -g.s[2 * e + 1]) : f2pack(g.s[2 * e], g.s[2 * e + 1]);
+    } else {                                         // pair (x, y): x' = x c - y s, y' = y c + x s
+      o.c[e] = f2pack(g.c[e], g.c[e]);
+      o.s[e] = f2pack(-g.s[e], g.s[e]);
+    }
+  }
+}
+
+// Norm and rotation of the row held as 8 elements a lane; the arithmetic of
+// norm8 and rotate8, product by product.
+__device__ __forceinline__ void norm_rope_row(const NormStoreArgs& a, const Pairs& g, bool norm, int hl, int src, float v[8]) {
+  uint64_t x[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[e] = f2pack(v[2 * e], v[2 * e + 1]);
+  if (norm) {
+    uint64_t ss2 = f2mul(x[0], x[0]);
+#pragma unroll
+    for (int e = 1; e < 4; ++e) ss2 = f2fma(x[e], x[e], ss2);
+    float s0, s1;
+    f2unpack(ss2, s0, s1);
+    float ss = s0 + s1;
+#pragma unroll
+    for (int k = 1; k < 16; k <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, k);
+    const float r = rsqrtf(ss * (1.0f / ns::D) + a.eps);
+    const uint64_t r2 = f2pack(r, r);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = f2mul(f2mul(x[e], r2), g.w[e]);
+  }
+  uint64_t y[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    float lo, hi;
+    f2unpack(x[e], lo, hi);
+    uint64_t p;                                      // the partners
+    if (a.neox) p = f2pack(__shfl_sync(0xffffffffu, lo, src), __shfl_sync(0xffffffffu, hi, src));
+    else p = f2pack(hi, lo);
+    y[e] = f2add(f2mul(x[e], g.c[e]), f2mul(p, g.s[e]));
+  }
+  const bool in = 8 * hl < a.rot;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) f2unpack(in ? y[e] : x[e], v[2 * e], v[2 * e + 1]);
 }
 
 template <int DT>
-__global__ void __launch_bounds__(ns::WARPS * 32) norm_store_fast_kernel(const __grid_constant__ NormStoreArgs a,
+__global__ void __launch_bounds__(ns::WARPS * 32, 3) norm_store_fast_kernel(const __grid_constant__ NormStoreArgs a,
                                                                          const __grid_constant__ FastItems f) {
   using namespace ns;
   __shared__ __align__(16) uint8_t stage_all[WARPS][16 * 128 + 128];
   uint8_t* stage = stage_all[warp_id()];
   const int lane = lane_id(), hl = lane & 15, half = lane >> 4;
-  const int64_t total = f.nq + f.nk + f.nv;
-  for (int64_t it = (int64_t)blockIdx.x * WARPS + warp_id(); it < total; it += (int64_t)gridDim.x * WARPS) {
+  const uint32_t total = f.nq + f.nk + f.nv, stride = gridDim.x * WARPS;
+  for (uint32_t it = blockIdx.x * WARPS + warp_id(); it < total; it += stride) {
     if (it < f.nq + f.nk) {
       const bool isq = it < f.nq;
-      const int64_t i = isq ? it : it - f.nq;
-      const int parts = isq ? f.pq : f.pk;
+      const uint32_t i = isq ? it : it - f.nq, parts = isq ? f.pq : f.pk;
       const int t = (int)(i / parts), H = isq ? a.Hq : a.Hkv;
       const int per = isq ? f.qr : 8;                    // rows of this item: per / 2 a half-warp
-      const int r0 = (int)(i - (int64_t)t * parts) * per;
+      const int r0 = (int)(i - t * parts) * per;
       const int rows = min(per, H - r0);
       int64_t pos = a.positions[t];
       if (pos < 0 || pos >= a.max_pos) {
@@ -418,38 +470,45 @@ __global__ void __launch_bounds__(ns::WARPS * 32) norm_store_fast_kernel(const _
       }
       const uint16_t* src = reinterpret_cast<const uint16_t*>(isq ? a.q : a.k) + (int64_t)t * (isq ? a.q_tok : a.k_tok) + 8 * hl;
       const int64_t hs = isq ? a.q_head : a.k_head;
+      // this half-warp's rows are `step` apart; a row past the last is read at the last one's place
+      const int64_t step = 2 * hs;
+      const uint16_t* sp = src + (int64_t)(r0 + half) * hs;
       uint4 raw[4];
 #pragma unroll
-      for (int x = 0; x < 4; ++x) raw[x] = *reinterpret_cast<const uint4*>(src + (int64_t)(r0 + min(2 * x + half, rows - 1)) * hs);
-      Angles g;
-      load_angles(a, pos, hl, g);
+      for (int x = 0; x < 4; ++x)
+        raw[x] = *reinterpret_cast<const uint4*>(2 * x + half < rows ? sp + x * step : src + (int64_t)(r0 + rows - 1) * hs);
+      Angles angles;
+      load_angles(a, pos, hl, angles);
       const void* wp = isq ? a.q_w : a.k_w;
       float w[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
       if (wp) widen8(load_raw8(wp, 8 * hl, isq ? a.qw_dt : a.kw_dt, false), isq ? a.qw_dt : a.kw_dt, w);
+      Pairs g;
+      make_pairs(a, angles, w, hl, g);
+      // the lane that holds this one's partners; lanes past the rotated part read themselves
+      const int lanes = a.rot >> 4, peer = hl >= 2 * lanes ? hl : hl < lanes ? hl + lanes : hl - lanes;
+      const int from = (lane & 16) | peer;
       if (isq) {
-        uint16_t* dst = reinterpret_cast<uint16_t*>(a.q_out) + (int64_t)t * a.qo_tok + 8 * hl;
-        for (int b = 0; b < rows; b += 8) {
-          uint4 cur[4];
-#pragma unroll
-          for (int x = 0; x < 4; ++x) cur[x] = raw[x];
-          if (b + 8 < rows) {
-#pragma unroll
-            for (int x = 0; x < 4; ++x) raw[x] = *reinterpret_cast<const uint4*>(src + (int64_t)(r0 + min(b + 8 + 2 * x + half, rows - 1)) * hs);
-          }
+        uint16_t* dp = reinterpret_cast<uint16_t*>(a.q_out) + (int64_t)t * a.qo_tok + (int64_t)(r0 + half) * a.qo_head + 8 * hl;
+        const int64_t dstep = 2 * a.qo_head;
+#pragma unroll 1
+        for (int left = rows - half; left > -half; left -= 8) {        // rows from this half's next one on
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
-            if (b + 2 * x >= rows) break;                // the same for both halves
+            if (left + half <= 2 * x) break;             // the same for both halves
             float v[8];
-            widen16<DT>(cur[x], v);
-            norm_rope_row<DT>(a, g, w, wp != nullptr, hl, v);
+            widen16<DT>(raw[x], v);
+            // the row eight further on takes its place, in flight while the others are worked on
+            if (left > 8 + 2 * x) raw[x] = *reinterpret_cast<const uint4*>(sp + (x + 4) * step);
+            norm_rope_row(a, g, wp != nullptr, hl, from, v);
             const uint4 packed = round8(v, DT);
-            const int r = b + 2 * x + half;
-            if (r < rows) *reinterpret_cast<uint4*>(dst + (int64_t)(r0 + r) * a.qo_head) = packed;
+            if (left > 2 * x) *reinterpret_cast<uint4*>(dp + x * dstep) = packed;
           }
+          sp += 4 * step;
+          dp += 4 * dstep;
         }
       } else {
         const int64_t slot = a.slots[t];
-        const int64_t blk = slot / a.c.block_size;
+        const int64_t blk = slot_page(slot, a.c.block_size, a.bs_log2);
         const int off = (int)(slot - blk * a.c.block_size);
         bool stored = slot >= 0;
         if (stored && a.c.num_blocks > 0 && blk >= a.c.num_blocks) {
@@ -462,7 +521,7 @@ __global__ void __launch_bounds__(ns::WARPS * 32) norm_store_fast_kernel(const _
           const int r = 2 * x + half;
           float v[8];
           widen16<DT>(raw[x], v);
-          norm_rope_row<DT>(a, g, w, wp != nullptr, hl, v);
+          norm_rope_row(a, g, wp != nullptr, hl, from, v);
           const uint4 packed = round8(v, DT);
           if (a.k_out && r < rows)
             *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.k_out) + (int64_t)t * a.ko_tok + (int64_t)(r0 + r) * a.ko_head + 8 * hl) = packed;
@@ -475,16 +534,16 @@ __global__ void __launch_bounds__(ns::WARPS * 32) norm_store_fast_kernel(const _
       }
       continue;
     }
-    const int64_t i = it - f.nq - f.nk;
+    const uint32_t i = it - f.nq - f.nk;
     if (a.c.v_mode != G9_V_Q8T) {
       // token rows: eight kv heads of a token
-      const int t = (int)(i / f.pv), r0 = (int)(i - (int64_t)t * f.pv) * 8, rows = min(8, a.Hkv - r0);
+      const int t = (int)(i / (uint32_t)f.pv), r0 = (int)(i - t * f.pv) * 8, rows = min(8, a.Hkv - r0);
       const uint16_t* src = reinterpret_cast<const uint16_t*>(a.v) + (int64_t)t * a.v_tok + 8 * hl;
       uint4 raw[4];
 #pragma unroll
       for (int x = 0; x < 4; ++x) raw[x] = *reinterpret_cast<const uint4*>(src + (int64_t)(r0 + min(2 * x + half, rows - 1)) * a.v_head);
       const int64_t slot = a.slots[t];
-      const int64_t blk = slot / a.c.block_size;
+      const int64_t blk = slot_page(slot, a.c.block_size, a.bs_log2);
       const int off = (int)(slot - blk * a.c.block_size);
       if (slot < 0) continue;
       if (a.c.num_blocks > 0 && blk >= a.c.num_blocks) {
@@ -509,8 +568,8 @@ __global__ void __launch_bounds__(ns::WARPS * 32) norm_store_fast_kernel(const _
       continue;
     }
     // ---- page-transposed V: (16 tokens, kv head) ----------------------------------
-    const int h = (int)(i % a.Hkv);
-    const int t0 = (int)(i / a.Hkv) * 16;
+    const int h = (int)(i % (uint32_t)a.Hkv);
+    const int t0 = (int)(i / (uint32_t)a.Hkv) * 16;
     const int bs = a.c.block_size;
     int64_t mine;
     const uint32_t cont = run_bits(a.slots, t0, a.T, a.c.num_blocks > 0 ? (int64_t)a.c.num_blocks * bs : INT64_MAX, mine);
@@ -519,7 +578,7 @@ __global__ void __launch_bounds__(ns::WARPS * 32) norm_store_fast_kernel(const _
       const int i0 = __ffs(heads) - 1;                   // the run's first token
       const int n = 1 + (i0 == 31 ? 0 : __ffs(~(cont >> (i0 + 1))) - 1);         // cont has a zero above bit 31 - i0
       const int64_t slot = __shfl_sync(0xffffffffu, mine, i0);
-      const int64_t blk = slot / bs;
+      const int64_t blk = slot_page(slot, bs, a.bs_log2);
       const int off = (int)(slot - blk * bs), sub = off & 15;
       const uint16_t* src = reinterpret_cast<const uint16_t*>(a.v) + (int64_t)(t0 + i0) * a.v_tok + (int64_t)h * a.v_head + 8 * hl;
       uint16_t* scales = reinterpret_cast<uint16_t*>(stage + 16 * 128);          // [block][16]
@@ -582,35 +641,43 @@ __global__ void __launch_bounds__(ns::WARPS * 32) norm_store_fast_kernel(const _
 // ---------------------------------------------------------------------------
 // read_kv: rows of the cache by slot, as 16- or 32-bit values
 // ---------------------------------------------------------------------------
+constexpr int RR = 4;
+
 struct ReadArgs {
   G9KvCache c;
   const int64_t* slots;
-  int N, Hkv, out_dt, v_src;                       // v_src: DT_F16 / DT_BF16 of 16-bit V rows
+  int bs_log2, N, Hkv, out_dt, v_src;                       // v_src: DT_F16 / DT_BF16 of 16-bit V rows
   int k_w8, v_w8, v_w16, v_rec16;                  // rows on 8- and 16-byte boundaries, records on 16
-  int64_t nrows;                                   // row items (two rows a warp); run items follow
-  int64_t nruns;
+  uint32_t nrows, nruns;                           // row items (2 * RR rows a warp); run items follow
   void* k_out; void* v_out;                        // [N, Hkv, 128]; v_out may be null
 };
 
-// elements 8 * hl .. + 7 of a Q8_0 row
-__device__ __forceinline__ void q8_lane(const uint8_t* row, int hl, bool w8, float v[8]) {
+// elements 8 * hl .. + 7 of a Q8_0 row as loaded, and their scale
+struct Q8Lane { uint64_t lo, hi; uint16_t d; };
+
+__device__ __forceinline__ Q8Lane q8_load(const uint8_t* row, int hl, bool w8) {
   const int blk = hl >> 2, o = blk * QBLOCK + 2 + 8 * (hl & 3);
-  uint64_t x;
-  float d;
+  Q8Lane x;
+  x.d = *reinterpret_cast<const uint16_t*>(row + blk * QBLOCK);
   if (w8) {
-    // the 8 values start 2, 4, 6 or 0 bytes into an aligned word: two words and a shift
+    // the 8 values start 2, 4, 6 or 0 bytes into an aligned word: that word and the next, which block 3 does not need
     const uint64_t* p = reinterpret_cast<const uint64_t*>(row + (o & ~7));
-    const int sh = (o & 7) * 8;
-    const uint64_t lo = p[0], hi = sh ? p[1] : 0;
-    x = sh ? lo >> sh | hi << (64 - sh) : lo;
-    d = half_of(*reinterpret_cast<const uint16_t*>(row + blk * QBLOCK));
+    x.lo = p[0];
+    x.hi = p[blk < 3];
   } else {
     const uint16_t* q = reinterpret_cast<const uint16_t*>(row + o);
-    x = (uint64_t)q[0] | (uint64_t)q[1] << 16 | (uint64_t)q[2] << 32 | (uint64_t)q[3] << 48;
-    d = half_of(*reinterpret_cast<const uint16_t*>(row + blk * QBLOCK));
+    x.lo = (uint64_t)q[0] | (uint64_t)q[1] << 16 | (uint64_t)q[2] << 32 | (uint64_t)q[3] << 48;
+    x.hi = 0;
   }
+  return x;
+}
+
+__device__ __forceinline__ void q8_values(const Q8Lane& x, int hl, bool w8, float v[8]) {
+  const int blk = hl >> 2, sh = w8 ? ((blk * QBLOCK + 2) & 7) * 8 : 0;
+  const uint64_t q = sh ? x.lo >> sh | x.hi << (64 - sh) : x.lo;
+  const float d = half_of(x.d);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = (float)(int8_t)(x >> (8 * e)) * d;
+  for (int e = 0; e < 8; ++e) v[e] = (float)(int8_t)(q >> (8 * e)) * d;
 }
 
 // Row items: half a warp reads one K or V row.  Run items: page-transposed V by
@@ -621,44 +688,63 @@ __global__ void __launch_bounds__(ns::WARPS * 32) read_kv_kernel(const __grid_co
   const int lane = lane_id(), hl = lane & 15;
   const int bs = a.c.block_size;
   const int64_t end = a.c.num_blocks > 0 ? (int64_t)a.c.num_blocks * bs : INT64_MAX;
-  const int64_t total = a.nrows + a.nruns, krows = (int64_t)a.N * a.Hkv;
-  for (int64_t it = (int64_t)blockIdx.x * WARPS + warp_id(); it < total; it += (int64_t)gridDim.x * WARPS) {
+  const uint32_t total = a.nrows + a.nruns, krows = (uint32_t)a.N * a.Hkv, stride = gridDim.x * WARPS;
+  for (uint32_t it = blockIdx.x * WARPS + warp_id(); it < total; it += stride) {
     if (it < a.nrows) {
-      const int64_t y = 2 * it + (lane >> 4);
-      const bool isv = y >= krows;
-      const int64_t r = isv ? y - krows : y;
-      if (r >= krows) continue;
-      const int64_t n = r / a.Hkv;
-      const int h = (int)(r - n * a.Hkv);
-      const int64_t slot = a.slots[n];
-      float v[8];
+      // RR rows a half-warp: their slots, then their cache rows, loaded together
+      uint32_t r[RR];
+      int64_t slot[RR];
+      bool isv[RR];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = 0.f;
-      if (slot >= end) raise_error(ERR_BAD_INDEX);
-      if (slot >= 0 && slot < end) {
-        const int64_t blk = slot / bs;
-        const int off = (int)(slot - blk * bs);
-        if (!isv) {
-          q8_lane(a.c.k + blk * a.c.k_page_stride + off * a.c.k_tok_stride + h * a.c.k_head_stride, hl, a.k_w8, v);
+      for (int k = 0; k < RR; ++k) {
+        const uint32_t y = (it * RR + k) * 2 + (lane >> 4);
+        isv[k] = y >= krows;
+        r[k] = isv[k] ? y - krows : y;
+        slot[k] = r[k] < krows ? a.slots[r[k] / (uint32_t)a.Hkv] : -1;
+      }
+      Q8Lane q[RR];
+      Raw8 w[RR];
+#pragma unroll
+      for (int k = 0; k < RR; ++k) {
+        q[k].lo = q[k].hi = 0;
+        q[k].d = 0;
+        w[k].a = w[k].b = make_uint4(0, 0, 0, 0);
+        if (slot[k] >= end) {
+          raise_error(ERR_BAD_INDEX);
+          slot[k] = -1;
+        }
+        if (slot[k] < 0) continue;
+        const int h = (int)(r[k] % (uint32_t)a.Hkv);
+        const int64_t blk = slot_page(slot[k], bs, a.bs_log2);
+        const int off = (int)(slot[k] - blk * bs);
+        if (!isv[k]) {
+          q[k] = q8_load(a.c.k + blk * a.c.k_page_stride + off * a.c.k_tok_stride + h * a.c.k_head_stride, hl, a.k_w8);
         } else if (a.c.v_mode == G9_V_Q8T) {             // records off 16-byte boundaries
           const uint8_t* rec = a.c.v + blk * a.c.v_page_stride + h * a.c.v_head_stride;
-          const float d = half_of(*reinterpret_cast<const uint16_t*>(rec + 2 * ((int64_t)(hl >> 2) * bs + off)));
-          const int8_t* q = reinterpret_cast<const int8_t*>(rec + 2 * (D / QK) * bs + (int64_t)8 * hl * bs + off);
+          q[k].d = *reinterpret_cast<const uint16_t*>(rec + 2 * ((int64_t)(hl >> 2) * bs + off));
+          const uint8_t* x = rec + 2 * (D / QK) * bs + (int64_t)8 * hl * bs + off;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = (float)q[(int64_t)e * bs] * d;
+          for (int e = 0; e < 8; ++e) q[k].lo |= (uint64_t)x[(int64_t)e * bs] << (8 * e);
         } else {
           const uint8_t* row = a.c.v + blk * a.c.v_page_stride + off * a.c.v_tok_stride + h * a.c.v_head_stride;
-          if (a.c.v_mode == G9_V_Q8) q8_lane(row, hl, a.v_w8, v);
-          else widen8(load_raw8(row, 8 * hl, a.v_src, a.v_w16), a.v_src, v);
+          if (a.c.v_mode == G9_V_Q8) q[k] = q8_load(row, hl, a.v_w8);
+          else w[k] = load_raw8(row, 8 * hl, a.v_src, a.v_w16);
         }
       }
-      const uint4 packed = round8(v, a.out_dt);
-      store8(isv ? a.v_out : a.k_out, r * D + 8 * hl, a.out_dt, true, v, packed);
+#pragma unroll
+      for (int k = 0; k < RR; ++k) {
+        if (r[k] >= krows) continue;
+        float v[8];
+        if (isv[k] && a.c.v_mode == G9_V_COPY16) widen8(w[k], a.v_src, v);
+        else q8_values(q[k], hl, isv[k] ? a.c.v_mode == G9_V_Q8 && a.v_w8 : a.k_w8, v);
+        const uint4 packed = round8(v, a.out_dt);
+        store8(isv[k] ? a.v_out : a.k_out, (int64_t)r[k] * D + 8 * hl, a.out_dt, true, v, packed);
+      }
       continue;
     }
-    const int64_t i = it - a.nrows;
-    const int h = (int)(i % a.Hkv);
-    const int t0 = (int)(i / a.Hkv) * 16;
+    const uint32_t i = it - a.nrows;
+    const int h = (int)(i % (uint32_t)a.Hkv);
+    const int t0 = (int)(i / (uint32_t)a.Hkv) * 16;
     int64_t mine;
     const uint32_t cont = run_bits(a.slots, t0, a.N, end, mine);
     const uint32_t live = __ballot_sync(0xffffffffu, mine >= 0);
@@ -674,7 +760,7 @@ __global__ void __launch_bounds__(ns::WARPS * 32) read_kv_kernel(const __grid_co
       s[0] = s[1] = make_uint4(0, 0, 0, 0);
       int sub = 0;
       if (slot >= 0) {
-        const int64_t blk = slot / bs;
+        const int64_t blk = slot_page(slot, bs, a.bs_log2);
         const int off = (int)(slot - blk * bs);
         sub = off & 15;
         const uint8_t* rec = a.c.v + blk * a.c.v_page_stride + (int64_t)h * a.c.v_head_stride;
@@ -741,6 +827,13 @@ static bool cache_ok(const G9KvCache& c) {
   return c.v && !(m & 1);
 }
 
+static int log2_or(int x) {
+  if (x & (x - 1)) return -1;
+  int n = 0;
+  while ((1 << n) < x) ++n;
+  return n;
+}
+
 static bool aligned(uintptr_t base, int64_t a, int64_t b, int64_t c, uintptr_t to) {
   return ((base | (uintptr_t)a | (uintptr_t)b | (uintptr_t)c) & (to - 1)) == 0;
 }
@@ -788,6 +881,7 @@ extern "C" cudaError_t gfx906_fa_norm_rope_store_kv(
   a.k_w8 = aligned((uintptr_t)cache->k, cache->k_page_stride, cache->k_tok_stride, cache->k_head_stride, 8);
   a.v_w8 = aligned((uintptr_t)cache->v, cache->v_page_stride, cache->v_tok_stride, cache->v_head_stride, 8);
   a.v_w16 = aligned((uintptr_t)cache->v, cache->v_page_stride, cache->v_tok_stride, cache->v_head_stride, 16);
+  a.bs_log2 = log2_or(cache->block_size);
   a.T = num_tokens; a.Hq = query ? num_heads_q : 0; a.Hkv = cache->num_heads_kv;
   a.rows = a.Hq + a.Hkv + (cache->v_mode != G9_V_NONE ? a.Hkv : 0);
   a.v_rec16 = cache->block_size % 16 == 0 &&
@@ -797,18 +891,20 @@ extern "C" cudaError_t gfx906_fa_norm_rope_store_kv(
   const bool fast = key_dtype != G9_DT_F32 && (!query || query_dtype == key_dtype) && (!withv || value_dtype == key_dtype) &&
                     a.k_vec && (!query || (a.q_vec && a.qo_vec)) && (!key_out || a.ko_vec) && (!withv || a.v_vec) && a.k_w8 &&
                     (cache->v_mode != G9_V_Q8 || a.v_w8) && (cache->v_mode != G9_V_COPY16 || a.v_w16) &&
-                    (cache->v_mode != G9_V_Q8T || cache->block_size % 16 == 0);
+                    (cache->v_mode != G9_V_Q8T || cache->block_size % 16 == 0) &&
+                    (int64_t)num_tokens * (a.Hq + 3 * (int64_t)a.Hkv) < 0x3fffffff;      // 32-bit item numbers
   if (fast) {
     FastItems f{};
-    // few tokens: 8 query rows a warp, so that more SMs have work; many: 16, which share the token's angles and weights
-    f.qr = (int64_t)num_tokens * a.Hq < (int64_t)sms * ns::WARPS * 32 ? 8 : 16;
+    // Few tokens: 8 query rows a warp, so that more SMs have work.  Many: a token's queries, which share its angles and the
+    // weights (16384 tokens of 48 + 8 heads, the whole call with its read back: 16 rows an item 204 us, a token's queries 193 us).
+    f.qr = (int64_t)num_tokens * a.Hq < (int64_t)sms * ns::WARPS * 32 ? 8 : (a.Hq + 7) / 8 * 8;
     f.pq = (a.Hq + f.qr - 1) / f.qr;
     f.pk = (a.Hkv + 7) / 8;
     f.pv = (a.Hkv + 7) / 8;
-    f.nq = (int64_t)num_tokens * f.pq;
-    f.nk = (int64_t)num_tokens * f.pk;
-    f.nv = !withv ? 0 : cache->v_mode == G9_V_Q8T ? (int64_t)((num_tokens + 15) / 16) * a.Hkv : (int64_t)num_tokens * f.pv;
-    const int64_t want = (f.nq + f.nk + f.nv + ns::WARPS - 1) / ns::WARPS, cap = (int64_t)sms * 32;
+    f.nq = num_tokens * f.pq;
+    f.nk = num_tokens * f.pk;
+    f.nv = !withv ? 0 : cache->v_mode == G9_V_Q8T ? (num_tokens + 15) / 16 * a.Hkv : num_tokens * f.pv;
+    const int64_t want = (int64_t)(f.nq + f.nk + f.nv + ns::WARPS - 1) / ns::WARPS, cap = (int64_t)sms * 32;
     const int grid = (int)(want < cap ? want : cap);
     if (key_dtype == G9_DT_F16) norm_store_fast_kernel<DT_F16><<<grid, ns::WARPS * 32, 0, stream>>>(a, f);
     else norm_store_fast_kernel<DT_BF16><<<grid, ns::WARPS * 32, 0, stream>>>(a, f);
@@ -832,6 +928,7 @@ extern "C" cudaError_t gfx906_fa_read_kv(const G9KvCache* cache, int value_dtype
     return cudaErrorInvalidValue;
   ReadArgs a{};
   a.c = *cache;
+  a.bs_log2 = log2_or(cache->block_size);
   a.slots = slots; a.N = num_rows; a.Hkv = cache->num_heads_kv; a.out_dt = out_dtype; a.v_src = value_dtype;
   a.k_out = key_out; a.v_out = value_out;
   a.k_w8 = aligned((uintptr_t)cache->k, cache->k_page_stride, cache->k_tok_stride, cache->k_head_stride, 8);
@@ -839,10 +936,11 @@ extern "C" cudaError_t gfx906_fa_read_kv(const G9KvCache* cache, int value_dtype
   a.v_w16 = aligned((uintptr_t)cache->v, cache->v_page_stride, cache->v_tok_stride, cache->v_head_stride, 16);
   a.v_rec16 = cache->block_size % 16 == 0 && aligned((uintptr_t)cache->v, cache->v_page_stride, cache->v_head_stride, 0, 16);
   const int64_t rows = (int64_t)num_rows * a.Hkv;
+  if (rows >= 0x3fffffff) return cudaErrorInvalidValue;                // 32-bit row numbers
   const bool runs = value_out && cache->v_mode == G9_V_Q8T && a.v_rec16;
-  a.nrows = (rows * (value_out && !runs ? 2 : 1) + 1) / 2;
-  a.nruns = runs ? (int64_t)((num_rows + 15) / 16) * a.Hkv : 0;
-  const int64_t want = (a.nrows + a.nruns + ns::WARPS - 1) / ns::WARPS, cap = (int64_t)ns_sms() * 32;
+  a.nrows = (uint32_t)((rows * (value_out && !runs ? 2 : 1) + 2 * RR - 1) / (2 * RR));
+  a.nruns = runs ? (uint32_t)((num_rows + 15) / 16) * a.Hkv : 0;
+  const int64_t want = (int64_t)(a.nrows + a.nruns + ns::WARPS - 1) / ns::WARPS, cap = (int64_t)ns_sms() * 32;
   read_kv_kernel<<<(int)(want < cap ? want : cap), ns::WARPS * 32, 0, stream>>>(a);
   return cudaGetLastError();
 }
