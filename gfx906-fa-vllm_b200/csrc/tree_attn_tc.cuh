@@ -304,8 +304,8 @@ __global__ void __launch_bounds__(tt::threads(NQ), 1) tree_tc_kernel(const __gri
   float* stat = reinterpret_cast<float*>(smem + smem_stat_off(NQ));          // [stream][m, l][row]
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + smem_bar_off(NQ));
   uint64_t *kfull = bars, *kempty = bars + 2, *vfull = bars + 4, *vempty = bars + 6, *qfull = bars + 8, *bs_ = bars + 10,
-           *bp = bars + 12, *bo = bars + 14, *bx = bars + 16, *by = bars + 17, *vraw = bars + 18;
-  int* misc = reinterpret_cast<int*>(bars + 26);     // 0: tensor memory, 1: abort, 2: poison, 4: b, 5: base, 8..23: scan
+           *bp = bars + 12, *bo = bars + 14, *bx = bars + 16, *by = bars + 17, *bpv = bars + 18, *vraw = bars + 20;
+  int* misc = reinterpret_cast<int*>(bars + 28);     // 0: tensor memory, 1: abort, 2: poison, 4: b, 5: base, 8..23: scan
   uint32_t* tilebad = reinterpret_cast<uint32_t*>(misc + 24);                // [8], a byte per 32 keys
 
   const TreeArgs& a = pp.a;
@@ -318,7 +318,7 @@ __global__ void __launch_bounds__(tt::threads(NQ), 1) tree_tc_kernel(const __gri
       // a tile is free when every stream that reads it is done: one (NQ = 1) or both
       mbar_init(&kfull[i], 4); mbar_init(&kempty[i], NQ);
       mbar_init(&vfull[i], 4); mbar_init(&vempty[i], NQ);
-      mbar_init(&bs_[i], 1); mbar_init(&bp[i], 128); mbar_init(&bo[i], 1);
+      mbar_init(&bs_[i], 1); mbar_init(&bp[i], 128); mbar_init(&bo[i], 1); mbar_init(&bpv[i], 1);
       mbar_init(&qfull[i], NQ == 1 ? 256 : 128);
     }
     for (int i = 0; i < 4 * GROUPS; ++i) mbar_init(&vraw[i], 32);
@@ -330,6 +330,9 @@ __global__ void __launch_bounds__(tt::threads(NQ), 1) tree_tc_kernel(const __gri
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&misc[0])));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
+  // Launched while the kernel before it in the stream finishes: nothing above reads or writes global memory.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;");
   // ---- this CTA's range of units ----------------------------------------------
   // Prefix sums of the sequences' units, NT sequences at a time; the sequence
   // that holds the range's first unit is found once the total is known, which
@@ -487,6 +490,7 @@ __global__ void __launch_bounds__(tt::threads(NQ), 1) tree_tc_kernel(const __gri
         if (shift) convert_rows<1>(raw + grp * 16 * PITCH, tile, 32 * w + 16 * grp);
         else convert_rows<0>(raw + grp * 16 * PITCH, tile, 32 * w + 16 * grp);
       }
+      fence_proxy_async();                   // the tensor core reads what this thread wrote
       __syncwarp();
     };
     if ((lw >> 2) < N) {
@@ -625,6 +629,7 @@ __global__ void __launch_bounds__(tt::threads(NQ), 1) tree_tc_kernel(const __gri
         }
       }
       if (hit) misc[2] = 1;
+      fence_proxy_async();
       __syncwarp();
       if (lane == 0) mbar_arrive(&vfull[t & 1]);
     }
@@ -638,15 +643,12 @@ __global__ void __launch_bounds__(tt::threads(NQ), 1) tree_tc_kernel(const __gri
     const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t tS = tmem + wi * 128 + lane_off, tO = tmem + 256 + wi * 128 + lane_off;
     const bool general = p.softcap > 0.f || !(p.scale > 0.f);
-    const bool leader = (tid & 127) == 0;    // issues the stream's MMAs
+    const bool leader = (tid & 127) == 96;   // issues the stream's MMAs; its warp has no rows of its own below 97 of them
     constexpr uint32_t kS = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
     constexpr uint32_t kPV = kS | (VF == G9_VFMT_Q8T ? 0u : 1u << 16);        // V by token rows: N-major
     const uint32_t qs = sQ + (NQ == 2 ? wi * TILE : 0);
-    // The proxy fence that lets the tensor core read what the loaders wrote stands here, after the wait for
-    // their arrivals, and not at their stores: there it would wait for their copies still in flight, a memory latency a tile.
     // Descriptors are advanced from one base each: the start address counts 16-byte units in the low bits.
     auto issue_s = [&](int n) {              // S = Q K(n)^T
-      fence_proxy_async();
       const uint64_t qd = sw128_desc(qs), kd = sw128_desc(sK + (n & 1) * TILE);
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) {
@@ -657,7 +659,6 @@ __global__ void __launch_bounds__(tt::threads(NQ), 1) tree_tc_kernel(const __gri
       tc_commit(&kempty[n & 1]);
     };
     auto issue_pv = [&](int n, bool first) { // O += P V(n)
-      fence_proxy_async();
       const uint32_t vs = sV + (n & 1) * TILE;
       const uint64_t vd = VF == G9_VFMT_Q8T ? sw128_desc(vs) : sw128_desc_mn(vs, TILE / 2);
 #pragma unroll
@@ -665,6 +666,7 @@ __global__ void __launch_bounds__(tt::threads(NQ), 1) tree_tc_kernel(const __gri
         const uint32_t off = (VF == G9_VFMT_Q8T ? (kk >> 2) * (TILE / 2) + (kk & 3) * 32 : kk * 2048) >> 4;
         tc_mma_ts(tmem + 256 + wi * 128, tmem + wi * 128 + kk * 8, vd + off, kPV, (!first || kk > 0) ? 1u : 0u);
       }
+      tc_commit(&bpv[wi]);
       tc_commit(&vempty[n & 1]);
     };
     constexpr int STEP = NQ == 1 ? 2 : 1;    // tiles between a stream's own
@@ -731,7 +733,8 @@ __global__ void __launch_bounds__(tt::threads(NQ), 1) tree_tc_kernel(const __gri
         tc_fence_after();
         issue_pv(n, j == j0);
         if (j + STEP < s.n) {
-          alive = mbar_wait(&kfull[(n + STEP) & 1], ((n + STEP) >> 1) & 1);
+          // the next scores overwrite the weights that this PV reads (only MMAs of one accumulator are sure to run in order)
+          alive = mbar_wait(&kfull[(n + STEP) & 1], ((n + STEP) >> 1) & 1) && mbar_wait(&bpv[wi], (cs - 1) & 1);
           if (!alive) return;
           tc_fence_after();
           issue_s(n + STEP);
@@ -783,16 +786,16 @@ __global__ void __launch_bounds__(tt::threads(NQ), 1) tree_tc_kernel(const __gri
           }
           tmem_wait_st();
         }
-        // Two passes over the scores, 64 at a time, so that a row never holds
-        // all 128 in registers: the maximum first, then the weights.
-        float mx = -INFINITY;
-#pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4) {
-          uint32_t x[1][32];
-          tmem_ld32(tS + q4 * 32, x[0]);
+        // 64 scores at a time, each half against the running maximum as it is then
+#pragma unroll 1
+        for (int hf = 0; hf < 2; ++hf) {
+          uint32_t x[2][32];
+          tmem_ld32(tS + hf * 64, x[0]);
+          tmem_ld32(tS + hf * 64 + 32, x[1]);
           tmem_wait_ld();
+          float mx = -INFINITY;
 #pragma unroll
-          for (int c = 0; c < 1; ++c) {
+          for (int c = 0; c < 2; ++c) {
             float m0 = __uint_as_float(x[c][0]), m1 = __uint_as_float(x[c][1]);
 #pragma unroll
             for (int e = 2; e < 30; e += 4) {
@@ -801,45 +804,58 @@ __global__ void __launch_bounds__(tt::threads(NQ), 1) tree_tc_kernel(const __gri
             }
             mx = fmax3(mx, fmax3(m0, m1, __uint_as_float(x[c][30])), __uint_as_float(x[c][31]));
           }
-        }
-        if (!general) mx *= a.scale_log2;    // scale > 0: the maximum commutes with it
-        float alpha = 1.f;
-        bool rescale = false;
-        if (mx != -INFINITY && (m == -INFINITY || mx > m + kRescale)) {
-          if (m != -INFINITY) {
-            alpha = fast_exp2(m - mx);
-            l *= alpha;
-            rescale = true;
+          if (!general) mx *= a.scale_log2;  // scale > 0: the maximum commutes with it
+          float alpha = 1.f;
+          bool rescale = false;
+          if (mx != -INFINITY && (m == -INFINITY || mx > m + kRescale)) {
+            if (m != -INFINITY) {
+              alpha = fast_exp2(m - mx);
+              l *= alpha;
+              rescale = true;
+            }
+            m = mx;
           }
-          m = mx;
-        }
-        if (__any_sync(0xffffffffu, rescale)) {
-          // S(j) complete: every earlier PV of this stream is in O
+          if (__any_sync(0xffffffffu, rescale)) {
+            // earlier tiles' PV are in O (the scores were issued after them); this tile's first half is still P
+            if (j != j0) {
 #pragma unroll 1
-          for (int c = 0; c < 4; ++c) {
-            uint32_t o[32];
-            tmem_ld32(tO + c * 32, o);
-            tmem_wait_ld();
+              for (int c = 0; c < 8; ++c) {
+                uint32_t o[16];
+                tmem_ld16(tO + c * 16, o);
+                tmem_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-            tmem_st32(tO + c * 32, o);
+                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                tmem_st16(tO + c * 16, o);
+              }
+            }
+            if (hf) {
+#pragma unroll 1
+              for (int c = 0; c < 4; ++c) {
+                uint32_t o[8];
+                tmem_wait_st();
+                tmem_ld8(tS + c * 8, o);
+                tmem_wait_ld();
+                const __half2 a2 = __float2half2_rn(alpha);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                  const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&o[e]), a2);
+                  o[e] = *reinterpret_cast<const uint32_t*>(&y);
+                }
+                tmem_st8(tS + c * 8, o);
+              }
+            }
           }
-        }
-        const float mu = m == -INFINITY ? 0.f : m;
-        const float sc = general ? 1.f : a.scale_log2;
-        const uint64_t sc2 = f2pack(sc, sc), nmu2 = f2pack(-mu, -mu);
-        uint64_t ls2[2] = {0ull, 0ull};
+          const float mu = m == -INFINITY ? 0.f : m;
+          const float sc = general ? 1.f : a.scale_log2;
+          const uint64_t sc2 = f2pack(sc, sc), nmu2 = f2pack(-mu, -mu);
+          uint64_t ls2[2] = {0ull, 0ull};
 #pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4) {
-          uint32_t x[32];
-          tmem_ld32(tS + q4 * 32, x);
-          tmem_wait_ld();
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
+          for (int c = 0; c < 4; ++c) {
             uint32_t pk[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-              const uint64_t y2 = f2fma(f2pack(__uint_as_float(x[c * 16 + 2 * e]), __uint_as_float(x[c * 16 + 2 * e + 1])), sc2, nmu2);
+              const uint64_t y2 = f2fma(f2pack(__uint_as_float(x[c >> 1][(c & 1) * 16 + 2 * e]),
+                                               __uint_as_float(x[c >> 1][(c & 1) * 16 + 2 * e + 1])), sc2, nmu2);
               float y0, y1;
               f2unpack(y2, y0, y1);
               y0 = fast_exp2(y0);
@@ -847,14 +863,14 @@ __global__ void __launch_bounds__(tt::threads(NQ), 1) tree_tc_kernel(const __gri
               ls2[e & 1] = f2add(ls2[e & 1], f2pack(y0, y1));
               pk[e] = pack_half2(y0, y1);
             }
-            // 32 weights take 16 columns: columns whose scores this row has read
-            tmem_st8(tS + q4 * 16 + c * 8, pk);
+            // 64 weights take 32 columns: columns whose scores this row has read
+            tmem_st8(tS + hf * 32 + c * 8, pk);
           }
+          float a0, a1, b0, b1;
+          f2unpack(ls2[0], a0, a1);
+          f2unpack(ls2[1], b0, b1);
+          l += (a0 + a1) + (b0 + b1);
         }
-        float a0, a1, b0, b1;
-        f2unpack(ls2[0], a0, a1);
-        f2unpack(ls2[1], b0, b1);
-        l += (a0 + a1) + (b0 + b1);
         tmem_wait_st();
         }                                    // rows past the group keep whatever S holds: O's rows are apart
         tc_fence_before();
@@ -984,6 +1000,7 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(const __grid_constant
   const int rb = blockIdx.x % row_blocks;
   const int rg = (blockIdx.x / row_blocks) % max_groups, b = blockIdx.x / row_blocks / max_groups;
   const int h = blockIdx.y;
+  asm volatile("griddepcontrol.wait;" ::: "memory");       // queued behind the attention kernel's start, runs after its end
   const TreeShape x = tree_shape<NQ>(a, b);
   if (rg >= x.groups) return;
   const int per = ((x.R + x.groups - 1) / x.groups + 31) & ~31;
@@ -1062,12 +1079,23 @@ cudaError_t launch_tree_tc_t(const TreeTcParams& pp, cudaStream_t stream) {
   auto kern = tree_tc_kernel<NQ, VF>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(NQ));
   if (e != cudaSuccess) return e;
-  kern<<<pp.NG * pp.Hkv, threads(NQ), smem_bytes(NQ), stream>>>(pp);
-  if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(pp.NG * pp.Hkv);
+  cfg.blockDim = dim3(threads(NQ));
+  cfg.dynamicSmemBytes = smem_bytes(NQ);
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if ((e = cudaLaunchKernelEx(&cfg, kern, pp)) != cudaSuccess) return e;
   if (pp.NG == 1) return cudaSuccess;        // nothing is cut
   const int rows = pp.a.p.seq_q * pp.a.G, groups = (rows + NQ * BM - 1) / (NQ * BM), blocks = pp.rc / 32;
-  tree_combine_kernel<NQ><<<dim3((unsigned)(pp.a.p.num_seqs * groups * blocks), pp.Hkv), 256, 0, stream>>>(pp, blocks, groups);
-  return cudaGetLastError();
+  cfg.gridDim = dim3((unsigned)(pp.a.p.num_seqs * groups * blocks), pp.Hkv);
+  cfg.blockDim = dim3(256);
+  cfg.dynamicSmemBytes = 0;
+  return cudaLaunchKernelEx(&cfg, tree_combine_kernel<NQ>, pp, blocks, groups);
 }
 
 }  // namespace g9
