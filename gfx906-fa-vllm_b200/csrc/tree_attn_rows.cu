@@ -178,8 +178,11 @@ TreePlan plan_tree(const G9AttnBatch& p) {
   if (off((uintptr_t)p.k_cache, p.k_page_stride, p.k_tok_stride, p.k_head_stride, 8)) return pl;
   const uintptr_t va = p.v_fmt == G9_VFMT_Q8 ? 8 : 16;
   if (off((uintptr_t)p.v_cache, p.v_page_stride, p.v_fmt == G9_VFMT_Q8T ? 0 : p.v_tok_stride, p.v_head_stride, va)) return pl;
-  const int64_t lim = 1 << 26;               // 16 rows' offsets are held in 32 bits
-  if (std::abs(p.k_tok_stride) >= lim || std::abs(p.v_tok_stride) >= lim || p.block_size > 32768) return pl;
+  // offsets inside a page are held in 32 bits, page strides in unsigned 32
+  const int64_t vt = p.v_fmt == G9_VFMT_Q8T ? 0 : p.v_tok_stride;
+  if (p.k_tok_stride < 0 || vt < 0 || p.block_size > 32768 || p.k_tok_stride * p.block_size > 0x3fffffff || vt * p.block_size > 0x3fffffff)
+    return pl;
+  if (p.k_page_stride < 0 || p.k_page_stride > 0xffffffffll || p.v_page_stride < 0 || p.v_page_stride > 0xffffffffll) return pl;
   const int64_t rows = (int64_t)p.seq_q * (p.num_heads_q / p.num_heads_kv);
   const int nq = rows > tt::BM ? 2 : 1;
   const int64_t groups = (rows + nq * tt::BM - 1) / (nq * tt::BM);
@@ -231,6 +234,10 @@ extern "C" cudaError_t gfx906_fa_tree_attention(const G9AttnBatch* batch, const 
   pp.Hkv = batch->num_heads_kv;
   pp.NG = pl.NG;
   pp.rc = pl.rc;
+  pp.kp = (uint32_t)batch->k_page_stride;
+  pp.vp = (uint32_t)batch->v_page_stride;
+  pp.kt = (int)batch->k_tok_stride;
+  pp.vt = batch->v_fmt == G9_VFMT_Q8T ? 0 : (int)batch->v_tok_stride;
   pp.bs_log2 = -1;
   if ((batch->block_size & (batch->block_size - 1)) == 0)
     for (pp.bs_log2 = 0; (1 << pp.bs_log2) < batch->block_size;) ++pp.bs_log2;

@@ -65,6 +65,8 @@ struct TreeTcParams {
   int Hkv, NG;
   int rc;                        // rows of a partial block (a multiple of 32)
   int bs_log2;                   // of the page size, -1: not a power of two
+  uint32_t kp, vp;               // byte strides of a page and of a token in 32 bits: one multiply an address
+  int kt, vt;
   int k_wide;                    // K rows may be copied as 16-byte pieces (even head counts)
   int out_vec;                   // output rows may be written 16 bytes at a time
   int* cum;                      // [num_seqs + 1] first unit of each sequence
@@ -246,7 +248,6 @@ __device__ __forceinline__ uint32_t ldg4_early(const void* p) {
   asm volatile("ld.global.L1::no_allocate.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
   return v;
 }
-__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 __device__ __forceinline__ uint4 ldg16_early(const void* p) {
   uint4 v;
   asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
@@ -404,11 +405,14 @@ __global__ void __launch_bounds__(tt::threads(NQ), 1) tree_tc_kernel(const __gri
 #pragma unroll
     for (int i = 0; i < 9; ++i) {
       const int y = i * 32 + lane, r = y / 9;
-      koff[i] = (int)((r & 15) * p.k_tok_stride) + (y - r * 9) * 16;
+      koff[i] = (r & 15) * pp.kt + (y - r * 9) * 16;
     }
+    // of a page-transposed record: this lane's scale word and its dims' values
+    const int vs_off = 2 * (lane >> 3) * bsz + 4 * (lane & 7), vq_off = 2 * (D / QK) * bsz + lane * bsz;
     TreeSeg s;
     s.n = 0;
     int pos = lw >> 2;                       // the next tile's place in the segment
+    const int32_t* bt = p.block_table;       // and the segment's row of the table
     // This warp's share of a tile: pages and in-page offsets of its two 16-key groups (page -1: none), keys inside the
     // sequence | checked << 8.
     struct Share { int ph0, ph1, of0, of1, info; };
@@ -420,10 +424,17 @@ __global__ void __launch_bounds__(tt::threads(NQ), 1) tree_tc_kernel(const __gri
       while (pos >= s.n) {
         pos -= s.n;
         if (!walk.next(a, s)) return;
+        bt = p.block_table + (int64_t)s.b * p.max_blocks;
       }
       const int k = (s.j + pos) * BN + 32 * w;
-      const int pg0 = pp.bs_log2 >= 0 ? k >> pp.bs_log2 : k / bsz, pg1 = pp.bs_log2 >= 0 ? (k + 16) >> pp.bs_log2 : (k + 16) / bsz;
-      const int32_t* bt = p.block_table + (int64_t)s.b * p.max_blocks;
+      int pg0, pg1;
+      if (pp.bs_log2 >= 0) {
+        pg0 = k >> pp.bs_log2;
+        pg1 = (k + 16) >> pp.bs_log2;
+      } else {
+        pg0 = k / bsz;
+        pg1 = (k + 16) / bsz;
+      }
       nxt.ph0 = bt[min(pg0, p.max_blocks - 1)];
       nxt.ph1 = bt[min(pg1, p.max_blocks - 1)];
       nxt.of0 = k - pg0 * bsz;
@@ -439,8 +450,8 @@ __global__ void __launch_bounds__(tt::threads(NQ), 1) tree_tc_kernel(const __gri
       if (valid > 0 && page_bad(p, cur.ph0)) bad = 1;
       if (valid > 16 && page_bad(p, cur.ph1)) bad |= 2;
       if (valid <= 16 || bad) {              // not every tile
-        if (valid == 0 || (bad & 1)) cur.ph0 = -1;
-        if (valid <= 16 || (bad & 2)) cur.ph1 = -1;
+        if (valid == 0 || (bad & 1)) { cur.ph0 = -1; cur.of0 = 0; }
+        if (valid <= 16 || (bad & 2)) { cur.ph1 = -1; cur.of1 = 0; }
         if (bad) {
           cur.info |= 256;
           if (lane == 0) raise_error(ERR_BAD_PAGE);
@@ -450,9 +461,9 @@ __global__ void __launch_bounds__(tt::threads(NQ), 1) tree_tc_kernel(const __gri
     };
     // 32 token rows of 136 bytes into the raw slot.  A page that is not there: page 0's bytes, whose scores are masked
     // and whose values are cleared.
-    auto load_rows = [&](const uint8_t* base, int64_t page_stride, int64_t tok_stride, bool wide) {
-      const uint8_t* s0 = base + (int64_t)max(cur.ph0, 0) * page_stride + (int64_t)(cur.ph0 < 0 ? 0 : cur.of0) * tok_stride;
-      const uint8_t* s1 = base + (int64_t)max(cur.ph1, 0) * page_stride + (int64_t)(cur.ph1 < 0 ? 0 : cur.of1) * tok_stride;
+    auto load_rows = [&](const uint8_t* base, uint32_t page_stride, int tok_stride, bool wide) {
+      const uint8_t* s0 = base + (uint64_t)(uint32_t)max(cur.ph0, 0) * page_stride + cur.of0 * tok_stride;
+      const uint8_t* s1 = base + (uint64_t)(uint32_t)max(cur.ph1, 0) * page_stride + cur.of1 * tok_stride;
       const uint32_t dst = smem_u32(raw) + lane * 16;
       if (wide) {
         // pieces 0..143 are the first group's rows
@@ -466,18 +477,10 @@ __global__ void __launch_bounds__(tt::threads(NQ), 1) tree_tc_kernel(const __gri
         }
       }
     };
-    // K rows of the settled tile; its V, needed a little later, on its way into L2
+    // K rows of the settled tile
     auto load_k = [&]() {
-      load_rows(kbase, p.k_page_stride, p.k_tok_stride, pp.k_wide);
+      load_rows(kbase, pp.kp, pp.kt, pp.k_wide);
       cp_async_commit();
-      const int ph = lane < 16 ? cur.ph0 : cur.ph1, of = lane < 16 ? cur.of0 : cur.of1;
-      const uint8_t* rec = vbase + (int64_t)max(ph, 0) * p.v_page_stride;
-      const int at = ph < 0 ? 0 : of;
-      if constexpr (VF == G9_VFMT_Q8T) prefetch_l2(rec + at + (lane & 15) * 136);      // a 16-token page's record
-      else {
-        prefetch_l2(rec + (int64_t)(at + (lane & 15)) * p.v_tok_stride);
-        if (DIRECT) prefetch_l2(rec + (int64_t)(at + (lane & 15)) * p.v_tok_stride + 128);
-      }
     };
     auto wait_empty = [&](uint64_t* bar, int t) {
       if (t >= ST && !mbar_wait(&bar[t & 1], ((t >> 1) - 1) & 1)) ok = false;
@@ -513,11 +516,12 @@ __global__ void __launch_bounds__(tt::threads(NQ), 1) tree_tc_kernel(const __gri
         // Scale word `lane`: keys 2 * (lane % 8), + 1 of block lane / 8.
 #pragma unroll
         for (int grp = 0; grp < 2; ++grp) {
-          const int ph = grp ? me.ph1 : me.ph0, at = ph < 0 ? 0 : grp ? me.of1 : me.of0;
-          const uint8_t* rec = vbase + (int64_t)max(ph, 0) * p.v_page_stride;
-          sc[grp] = ldg4_early(rec + 2 * ((lane >> 3) * bsz + at) + 4 * (lane & 7));
+          const int ph = grp ? me.ph1 : me.ph0, at = grp ? me.of1 : me.of0;
+          const uint8_t* rec = vbase + (uint64_t)(uint32_t)max(ph, 0) * pp.vp;
+          sc[grp] = ldg4_early(rec + vs_off + 2 * at);
+          const uint8_t* val = rec + vq_off + at;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) q[grp][i] = ldg16_early(rec + 2 * (D / QK) * bsz + (int64_t)(lane + 32 * i) * bsz + at);
+          for (int i = 0; i < 4; ++i) q[grp][i] = ldg16_early(val + i * 32 * bsz);
         }
       } else if constexpr (DIRECT) {
         // 16-bit rows go straight into the operand tile; rows of a page that is not there are zeroed
@@ -526,12 +530,12 @@ __global__ void __launch_bounds__(tt::threads(NQ), 1) tree_tc_kernel(const __gri
 #pragma unroll
         for (int grp = 0; grp < 2; ++grp) {
           const int ph = grp ? me.ph1 : me.ph0, at = grp ? me.of1 : me.of0;
-          const uint8_t* src = vbase + (int64_t)ph * p.v_page_stride + (int64_t)at * p.v_tok_stride + 16 * c;
+          const uint8_t* src = vbase + (uint64_t)(uint32_t)ph * pp.vp + at * pp.vt + 16 * c;
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const int r = 2 * i + (lane >> 4), key = 32 * w + 16 * grp + r;
             uint8_t* to = vtile + (c >> 3) * (TILE / 2) + key * 128 + (((c & 7) ^ (key & 7)) << 4);
-            if (ph >= 0) cp_async16(smem_u32(to), src + (int64_t)r * p.v_tok_stride);
+            if (ph >= 0) cp_async16(smem_u32(to), src + r * pp.vt);
             else *reinterpret_cast<uint4*>(to) = make_uint4(0, 0, 0, 0);
           }
         }
@@ -546,7 +550,7 @@ __global__ void __launch_bounds__(tt::threads(NQ), 1) tree_tc_kernel(const __gri
       convert(smem + (t & 1) * TILE, odd);
       if (lane == 0) mbar_arrive(&kfull[t & 1]);
       if (VF == G9_VFMT_Q8) {                // token-row V takes the slot in turn
-        load_rows(vbase, p.v_page_stride, p.v_tok_stride, false);
+        load_rows(vbase, pp.vp, pp.vt, false);
         cp_async_commit();
       } else if (more) {
         settle(t + GROUPS);

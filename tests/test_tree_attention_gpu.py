@@ -253,3 +253,91 @@ def test_refusals():
         with pytest.raises(RuntimeError):
             call(**over)
     call()
+
+
+def test_many_short_sequences():
+    """More sequences than a prefix-sum chunk, some without drafts."""
+    rng = np.random.default_rng(20)
+    n_q = [int(x) for x in rng.integers(0, 5, 1100)]
+    lens = [n + int(x) for n, x in zip(n_q, rng.integers(0, 40, 1100))]
+    check(TreeCase(lens, n_q, 4, 2, "q8t", seed=20), "1100 sequences")
+
+
+@pytest.mark.parametrize("v_fmt", ["q8t", "f16"])
+@pytest.mark.parametrize("rows", [16, 40])
+def test_scores_that_jump(rows, v_fmt):
+    """Every 64 keys score at a level of their own, up to 15 nats apart, so that the running maximum rises by more than the
+    lazy threshold in first and second halves of tiles: the accumulator, and weights already written, are scaled down.
+    (15 nats of score err by 15 * 2^-12 from the keys' rounding, the same way in every element: 0.4 %.)"""
+    import gfx906_fa
+    B, L = 60, 1500
+    case = TreeCase([L] * B, [rows] * B, 6, 1, v_fmt, seed=21, dtype=torch.float16)
+    g = torch.Generator().manual_seed(1)
+    level = (torch.rand((B, L // 64 + 1), generator=g) * 1.3).repeat_interleave(64, 1)[:, :L]
+    key = (level.reshape(-1, 1, 1) * torch.ones(B * L, 1, 128)).half()
+    val = torch.randn((B * L, 1, 128), generator=g).half()
+    pos = torch.arange(L)
+    slots = (case.block_table[:, pos // 16].long() * 16 + pos % 16).flatten()
+    gfx906_fa.store_kv(key.to(dev), val.to(dev), slots.to(dev), case.k_cache, case.v_cache, 3 if v_fmt == "q8t" else 1)
+    case.q = (1 + 0.05 * torch.randn(case.q.shape, generator=g)).half().to(dev)
+    check(case, "jumps")
+
+
+def test_lengths_past_the_table_or_the_bound_are_clamped():
+    case = TreeCase([300, 200], [4, 4], 12, 2, "q8t", seed=22)
+    short = TreeCase([304, 200], [4, 4], 12, 2, "q8t", seed=22)
+    lens = short.lens.clone()
+    lens[0] = 5000                                     # the table holds 19 pages: 304 keys
+    case = short
+    case.lens = lens
+    assert_close(case.run().float().cpu().numpy(), case.reference(), what="clamped to the table")
+
+
+@pytest.mark.parametrize("bits", [1, 2])
+def test_caches_the_tensor_core_kernel_cannot_read(bits):
+    """Rows on 2-byte boundaries only."""
+    case = TreeCase([210, 40], [9, 5], 12, 2, "q8", seed=23)
+    ref = case.reference()
+    for name in ("k_cache", "v_cache"):
+        c = getattr(case, name)
+        wide = torch.zeros((*c.shape[:3], 138), dtype=torch.uint8, device=dev)
+        wide[..., :136] = c
+        if bits == 1 or name == "k_cache":
+            setattr(case, name, wide[..., :136])
+    assert_close(case.run().float().cpu().numpy(), ref, what="2-byte rows")
+
+
+def test_backend_cache_views():
+    """The views of one vLLM allocation: K rows and V records share each page's K half."""
+    import gfx906_fa
+    for v_fmt, mode, fmt in (("q8_0", 3, "q8t"), ("fp16", 1, "bf16")):
+        case = TreeCase([500, 77], [12, 7], 16, 8, fmt, seed=24)
+        ref = case.reference()
+        kv = torch.full((case.NB, 2, 16, 8, 128), float("nan"), dtype=torch.bfloat16, device=dev)
+        k, v = gfx906_fa_paged.kv_cache_views(kv, v_fmt)
+        k.copy_(case.k_cache)
+        v.copy_(case.v_cache)
+        case.k_cache, case.v_cache = k, v
+        assert_close(case.run().float().cpu().numpy(), ref, what=v_fmt)
+        assert gfx906_fa.device_error(True) == 0
+
+
+def test_a_visible_key_that_is_not_a_number_shows():
+    import gfx906_fa
+    case = TreeCase([700], [6], 6, 1, "q8t", seed=25)
+    slot = int(case.block_table[0, 3]) * 16 + 5
+    case.k_cache.view(-1, 136)[slot, :2] = 255         # a NaN scale in the context
+    assert np.isnan(case.run().float().cpu().numpy()).all()
+    assert gfx906_fa.device_error(True) == 0
+
+
+def test_zero_and_negative_scale():
+    for scale in (0.0, -0.05):
+        case = TreeCase([333, 20], [6, 9], 12, 2, "q8t", seed=26)
+        import gfx906_fa
+        out = gfx906_fa.tree_attention(case.q, case.k_cache, case.v_cache, case.bt, case.lens, case.start, case.mask, 9, 333, scale)
+        type(case).scale = property(lambda self, s=scale: s)
+        try:
+            assert_close(out.float().cpu().numpy(), case.reference(), what=f"scale {scale}")
+        finally:
+            del type(case).scale
