@@ -202,7 +202,10 @@ __device__ __forceinline__ int clean2(uint32_t& w, bool dead0, bool dead1) {
 static __device__ __noinline__ bool tree_poisoned(const TreeArgs& a, const TreeSeg& s, int h, const int32_t* row, int lo) {
   const G9AttnBatch& p = a.p;
   for (int j = s.j; j < s.j + s.n; ++j) {
-    if (!tree_checked(a, s, j * tt::BN)) continue;
+    bool checked = tree_checked(a, s, j * tt::BN);         // or a page of it is not there
+    for (int k = j * tt::BN; !checked && k < min(s.L, (j + 1) * tt::BN); k += 16)
+      checked = page_bad(p, p.block_table[(int64_t)s.b * p.max_blocks + k / p.block_size]);
+    if (!checked) continue;
     for (int k = j * tt::BN; k < min(s.L, (j + 1) * tt::BN); ++k) {
       if (!(tree_sees(row, a.words, s.nq, s.ctx, lo, k) & 1u)) continue;
       const int phys = p.block_table[(int64_t)s.b * p.max_blocks + k / p.block_size];

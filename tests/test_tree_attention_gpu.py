@@ -341,3 +341,19 @@ def test_zero_and_negative_scale():
             assert_close(out.float().cpu().numpy(), case.reference(), what=f"scale {scale}")
         finally:
             del type(case).scale
+
+
+@pytest.mark.parametrize("v_fmt", ["q8t", "f16"])
+def test_pages_past_four_gigabytes(v_fmt):
+    """The same pages at the end of a cache whose byte offsets need more than 32 bits."""
+    case = TreeCase([900, 130], [16, 9], 48, 8, v_fmt, seed=27, dtype=torch.float16)
+    ref = case.reference()
+    kv = torch.empty((72000, 2, 16, 8, 128), dtype=torch.float16, device=dev)         # 65536 bytes a page
+    k, v = gfx906_fa_paged.kv_cache_views(kv, "q8_0" if v_fmt == "q8t" else "fp16")
+    first = kv.shape[0] - case.NB
+    assert first * 65536 > 2 ** 32
+    k[first:] = case.k_cache
+    v[first:] = case.v_cache
+    case.k_cache, case.v_cache = k, v
+    case.bt = torch.where(case.bt >= 0, case.bt + first, case.bt)
+    assert_close(case.run().float().cpu().numpy(), ref, what="far pages")

@@ -448,3 +448,31 @@ def test_copy_pages_odd_sizes_strides_and_refusals():
                 ([base.view(6, 3, 334)[:, :, :300]], one, four), ([base[:, 1:1000]], one, four)):
         with pytest.raises(RuntimeError):
             gfx906_fa.copy_pages(*bad)
+
+
+@pytest.mark.parametrize("mode", [1, 3])
+def test_slots_past_four_gigabytes(mode):
+    """Store, read back, move and copy at the end of a cache whose byte offsets need more than 32 bits."""
+    import gfx906_fa
+    from gfx906_fa_paged import kv_cache_views
+    kv = torch.empty((72000, 2, BS, 8, D), dtype=torch.bfloat16, device=dev)
+    k, v = kv_cache_views(kv, "q8_0" if mode == 3 else "fp16")
+    qkv, w, pos, _, _ = store_case(40, 8, 8, torch.bfloat16, seed=5)
+    d = qkv.to(dev)
+    slots = torch.arange(71990 * BS + 3, 71990 * BS + 43)
+    ko = torch.empty((40, 8, D), dtype=torch.bfloat16, device=dev)
+    gfx906_fa.norm_rope_store_kv(d[:, :8], d[:, 8:16], d[:, 16:], w[0].to(dev), w[1].to(dev), 1e-6, pos.to(dev),
+                                 cos_sin(4000, 128).float().to(dev), True, slots.to(dev), k, v, mode, key_out=ko)
+    rows = np.zeros((3, BS, 8, 136), np.uint8)
+    O.reshape_and_cache(to_np(ko), slots.numpy() - 71990 * BS, rows, dtype="bf16")
+    want = torch.from_numpy(dequant_rows(rows.reshape(-1, 8, 136)[3:43])).float().to(dev)
+    got_k, got_v = gfx906_fa.read_kv(k, v, slots.to(dev), torch.float32)
+    assert torch.equal(got_k, want)
+    if mode == 1:
+        assert torch.equal(got_v, qkv[:, 16:].float().to(dev))
+    gfx906_fa.move_kv([k], [v], slots[20:30].to(dev), slots[:10].to(dev), 10)
+    moved = gfx906_fa.read_kv(k, v, slots[:10].to(dev), torch.float32)
+    assert torch.equal(moved[0], want[20:30]) and torch.equal(moved[1], got_v[20:30])
+    gfx906_fa.copy_pages([kv], torch.tensor([71991], device=dev), torch.tensor([71999], device=dev))
+    assert torch.equal(kv.view(torch.uint8)[71999], kv.view(torch.uint8)[71991])
+    assert gfx906_fa.device_error(True) == 0
