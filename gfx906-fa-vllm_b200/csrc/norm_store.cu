@@ -9,9 +9,13 @@
 //
 // Half a warp holds a row, 8 elements a lane, so every row is one 16-byte
 // load per lane, the mean of squares four shuffles and a Q8_0 block's maximum
-// two.  All arithmetic is fp32.  Bound by HBM: queries and keys are read and
-// written once, where separate norm, rotation and store passes move them
-// three times.
+// two.  All arithmetic is fp32.  Queries and keys are read and written once,
+// where separate norm, rotation and store passes move them three times.
+// 16384 tokens of 48 + 8 heads (505 MB): 140 us, 3.6 TB/s.  Bound by what 24
+// warps an SM keep in flight between their dependent loads (position, angles,
+// rows), with half the issue slots taken: 127 instructions a pair of query rows.
+#include <cstdlib>
+
 #include "common.cuh"
 #include "gfx906_fa_b200.h"
 #include "tcgen05.cuh"
@@ -166,6 +170,34 @@ __device__ __forceinline__ uint2 quant8(const float v[8], uint16_t& scale) {
   }
   scale = __half_as_ushort(__float2half_rn(d));
   return make_uint2(w[0], w[1]);
+}
+
+// The same for elements that are fp16 or bf16 values, without the division
+// routine and the conversions: amax / 127 as a product with 1/127 and one
+// residual step, and the nearest integer by adding 1.5 * 2^23 (ties to even),
+// both exact for such values (the KV store's tests check every 16-bit maximum).
+__device__ __forceinline__ uint2 quant8_16bit(const float v[8], uint16_t& scale) {
+  float amax = fabsf(v[0]);
+#pragma unroll
+  for (int e = 1; e < 8; ++e) amax = fmaxf(amax, fabsf(v[e]));
+  amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+  amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+  constexpr float kInv127 = 1.0f / 127.0f;
+  const float y = __fmul_rn(amax, kInv127);
+  const float d = fmaf(fmaf(-y, 127.0f, amax), kInv127, y);
+  const float id = d > 0.0f ? __frcp_rn(d) : 0.0f;
+  constexpr float kMagic = 12582912.0f;
+  uint32_t b[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    float r = __fadd_rn(__fmul_rn(v[e], id), kMagic);
+    r = r == r ? r : kMagic;                         // 0 * inf: a scale that underflowed
+    r = fminf(fmaxf(r, kMagic - 128.0f), kMagic + 127.0f);
+    b[e] = __float_as_uint(r);
+  }
+  scale = __half_as_ushort(__float2half_rn(d));
+  return make_uint2(__byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410),
+                    __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410));
 }
 
 // cos / sin of this lane's 8 elements.  NeoX: element e pairs with e +- rot/2;
@@ -351,7 +383,9 @@ __global__ void __launch_bounds__(ns::WARPS * 32) norm_store_kernel(const __grid
 
 // ---------------------------------------------------------------------------
 // 16-bit tensors of one type on 16-byte rows, 8-byte cache rows: what a model
-// serves.  Queries, keys and values are separate warp items, so that no warp
+// serves.  Three CTAs an SM at 80 registers: two took 228 us where three took
+// 193 for 16384 tokens and their read back; four spill (175 against 179 now, but
+// 37 against 29 at 2111 tokens).  Queries, keys and values are separate warp items, so that no warp
 // carries another operand's code: a query item is QR rows of a token (their
 // angles loaded once), a key item its kv heads, a value item a run of slots
 // (page-transposed) or a token's heads.
@@ -413,7 +447,8 @@ __device__ __forceinline__ void make_pairs(const NormStoreArgs& a, const Angles&
 }
 
 // Norm and rotation of the row held as 8 elements a lane; the arithmetic of
-// norm8 and rotate8, product by product.
+// norm8 and rotate8, product by product.  FULL: every element is rotated.
+template <bool NEOX, bool FULL>
 __device__ __forceinline__ void norm_rope_row(const NormStoreArgs& a, const Pairs& g, bool norm, int hl, int src, float v[8]) {
   uint64_t x[4];
 #pragma unroll
@@ -438,16 +473,16 @@ __device__ __forceinline__ void norm_rope_row(const NormStoreArgs& a, const Pair
     float lo, hi;
     f2unpack(x[e], lo, hi);
     uint64_t p;                                      // the partners
-    if (a.neox) p = f2pack(__shfl_sync(0xffffffffu, lo, src), __shfl_sync(0xffffffffu, hi, src));
+    if (NEOX) p = f2pack(__shfl_sync(0xffffffffu, lo, src), __shfl_sync(0xffffffffu, hi, src));
     else p = f2pack(hi, lo);
     y[e] = f2add(f2mul(x[e], g.c[e]), f2mul(p, g.s[e]));
   }
-  const bool in = 8 * hl < a.rot;
+  const bool in = FULL || 8 * hl < a.rot;
 #pragma unroll
   for (int e = 0; e < 4; ++e) f2unpack(in ? y[e] : x[e], v[2 * e], v[2 * e + 1]);
 }
 
-template <int DT>
+template <int DT, bool NEOX, bool FULL>
 __global__ void __launch_bounds__(ns::WARPS * 32, 3) norm_store_fast_kernel(const __grid_constant__ NormStoreArgs a,
                                                                          const __grid_constant__ FastItems f) {
   using namespace ns;
@@ -469,9 +504,9 @@ __global__ void __launch_bounds__(ns::WARPS * 32, 3) norm_store_fast_kernel(cons
         pos = 0;
       }
       const uint16_t* src = reinterpret_cast<const uint16_t*>(isq ? a.q : a.k) + (int64_t)t * (isq ? a.q_tok : a.k_tok) + 8 * hl;
-      const int64_t hs = isq ? a.q_head : a.k_head;
+      const int64_t hs = isq ? a.q_head : a.k_head;        // below 2^24
       // this half-warp's rows are `step` apart; a row past the last is read at the last one's place
-      const int64_t step = 2 * hs;
+      const int step = (int)(2 * hs);
       const uint16_t* sp = src + (int64_t)(r0 + half) * hs;
       uint4 raw[4];
 #pragma unroll
@@ -489,7 +524,7 @@ __global__ void __launch_bounds__(ns::WARPS * 32, 3) norm_store_fast_kernel(cons
       const int from = (lane & 16) | peer;
       if (isq) {
         uint16_t* dp = reinterpret_cast<uint16_t*>(a.q_out) + (int64_t)t * a.qo_tok + (int64_t)(r0 + half) * a.qo_head + 8 * hl;
-        const int64_t dstep = 2 * a.qo_head;
+        const int dstep = (int)(2 * a.qo_head);
 #pragma unroll 1
         for (int left = rows - half; left > -half; left -= 8) {        // rows from this half's next one on
 #pragma unroll
@@ -499,7 +534,7 @@ __global__ void __launch_bounds__(ns::WARPS * 32, 3) norm_store_fast_kernel(cons
             widen16<DT>(raw[x], v);
             // the row eight further on takes its place, in flight while the others are worked on
             if (left > 8 + 2 * x) raw[x] = *reinterpret_cast<const uint4*>(sp + (x + 4) * step);
-            norm_rope_row(a, g, wp != nullptr, hl, from, v);
+            norm_rope_row<NEOX, FULL>(a, g, wp != nullptr, hl, from, v);
             const uint4 packed = round8(v, DT);
             if (left > 2 * x) *reinterpret_cast<uint4*>(dp + x * dstep) = packed;
           }
@@ -521,13 +556,13 @@ __global__ void __launch_bounds__(ns::WARPS * 32, 3) norm_store_fast_kernel(cons
           const int r = 2 * x + half;
           float v[8];
           widen16<DT>(raw[x], v);
-          norm_rope_row(a, g, wp != nullptr, hl, from, v);
+          norm_rope_row<NEOX, FULL>(a, g, wp != nullptr, hl, from, v);
           const uint4 packed = round8(v, DT);
           if (a.k_out && r < rows)
             *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.k_out) + (int64_t)t * a.ko_tok + (int64_t)(r0 + r) * a.ko_head + 8 * hl) = packed;
           if (!stored) continue;                         // the same for the warp
           uint16_t scale;
-          const uint2 q = quant8(v, scale);
+          const uint2 q = quant8_16bit(v, scale);
           uint8_t* dst = a.c.k + blk * a.c.k_page_stride + off * a.c.k_tok_stride + (int64_t)(r0 + r) * a.c.k_head_stride;
           write_q8_row(dst, q, scale, hl, r < rows, true, stage + half * RB);
         }
@@ -561,7 +596,7 @@ __global__ void __launch_bounds__(ns::WARPS * 32, 3) norm_store_fast_kernel(cons
           float v[8];
           widen16<DT>(raw[x], v);
           uint16_t scale;
-          const uint2 q = quant8(v, scale);
+          const uint2 q = quant8_16bit(v, scale);
           write_q8_row(dst, q, scale, hl, r < rows, true, stage + half * RB);
         }
       }
@@ -594,7 +629,7 @@ __global__ void __launch_bounds__(ns::WARPS * 32, 3) norm_store_fast_kernel(cons
           float v[8];
           widen16<DT>(raw[x], v);
           uint16_t scale;
-          const uint2 q = quant8(v, scale);
+          const uint2 q = quant8_16bit(v, scale);
           if (k < n) {
             *reinterpret_cast<uint2*>(stage + (sub + k) * 128 + 8 * hl) = q;
             if ((hl & 3) == 0) scales[(hl >> 2) * 16 + sub + k] = scale;
@@ -680,7 +715,7 @@ __device__ __forceinline__ void q8_values(const Q8Lane& x, int hl, bool w8, floa
   for (int e = 0; e < 8; ++e) v[e] = (float)(int8_t)(q >> (8 * e)) * d;
 }
 
-// Row items: half a warp reads one K or V row.  Run items: page-transposed V by
+// 16384 rows of 8 heads: 37 us for 103 MB.  Row items: half a warp reads RR rows.  Run items: page-transposed V by
 // runs of slots (run_bits): a lane takes 4 dims x 16 tokens as four 16-byte
 // loads, whatever part of the 16 the run covers.
 __global__ void __launch_bounds__(ns::WARPS * 32) read_kv_kernel(const __grid_constant__ ReadArgs a) {
@@ -892,7 +927,8 @@ extern "C" cudaError_t gfx906_fa_norm_rope_store_kv(
                     a.k_vec && (!query || (a.q_vec && a.qo_vec)) && (!key_out || a.ko_vec) && (!withv || a.v_vec) && a.k_w8 &&
                     (cache->v_mode != G9_V_Q8 || a.v_w8) && (cache->v_mode != G9_V_COPY16 || a.v_w16) &&
                     (cache->v_mode != G9_V_Q8T || cache->block_size % 16 == 0) &&
-                    (int64_t)num_tokens * (a.Hq + 3 * (int64_t)a.Hkv) < 0x3fffffff;      // 32-bit item numbers
+                    (int64_t)num_tokens * (a.Hq + 3 * (int64_t)a.Hkv) < 0x3fffffff &&    // 32-bit item numbers
+                    std::abs(a.q_head) < (1 << 24) && std::abs(a.k_head) < (1 << 24) && std::abs(a.qo_head) < (1 << 24);
   if (fast) {
     FastItems f{};
     // Few tokens: 8 query rows a warp, so that more SMs have work.  Many: a token's queries, which share its angles and the
@@ -906,9 +942,17 @@ extern "C" cudaError_t gfx906_fa_norm_rope_store_kv(
     f.nv = !withv ? 0 : cache->v_mode == G9_V_Q8T ? (num_tokens + 15) / 16 * a.Hkv : num_tokens * f.pv;
     const int64_t want = (int64_t)(f.nq + f.nk + f.nv + ns::WARPS - 1) / ns::WARPS, cap = (int64_t)sms * 32;
     const int grid = (int)(want < cap ? want : cap);
-    if (key_dtype == G9_DT_F16) norm_store_fast_kernel<DT_F16><<<grid, ns::WARPS * 32, 0, stream>>>(a, f);
-    else norm_store_fast_kernel<DT_BF16><<<grid, ns::WARPS * 32, 0, stream>>>(a, f);
-    return cudaGetLastError();
+    auto launch = [&](auto kern) {
+      kern<<<grid, ns::WARPS * 32, 0, stream>>>(a, f);
+      return cudaGetLastError();
+    };
+    const bool full = rot_dim == 128;
+    if (key_dtype == G9_DT_F16) {
+      if (a.neox) return full ? launch(norm_store_fast_kernel<DT_F16, true, true>) : launch(norm_store_fast_kernel<DT_F16, true, false>);
+      return full ? launch(norm_store_fast_kernel<DT_F16, false, true>) : launch(norm_store_fast_kernel<DT_F16, false, false>);
+    }
+    if (a.neox) return full ? launch(norm_store_fast_kernel<DT_BF16, true, true>) : launch(norm_store_fast_kernel<DT_BF16, true, false>);
+    return full ? launch(norm_store_fast_kernel<DT_BF16, false, true>) : launch(norm_store_fast_kernel<DT_BF16, false, false>);
   }
   // other types, alignments and page sizes; a half-warp a row when rows are few, else BATCH rows share a token's angles
   a.rpw = (int64_t)num_tokens * a.rows < (int64_t)sms * ns::WARPS * 2 * ns::BATCH ? 1 : ns::BATCH;
