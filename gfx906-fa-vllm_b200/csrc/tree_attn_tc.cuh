@@ -5,9 +5,10 @@
 //
 // The rows of one kv head of one sequence are its drafts times the GQA group
 // (row = t * G + g): 16 drafts at GQA 6 are 96 rows, so one pass over the cache
-// carries 4 * 96 FLOP per cached byte and the pass is bound by HBM and by the
-// issue slots of dequantisation and softmax together, where a warp-level MMA
-// would be bound by its own rate and a dequantised staging copy by traffic.
+// carries 512 * 96 FLOP for the 272 bytes of a key and its Q8_0 value.  That is 180 FLOP a
+// byte, near the balance of HBM and tensor cores: a warp-level MMA would be
+// bound by its own rate, a dequantised staging copy by traffic, and what
+// this kernel has to fit beside both is dequantisation and softmax.
 //
 // Work: the key tiles (128 keys) of all (sequence, row group) items laid end
 // to end are cut into NG equal ranges; CTA (g, h) computes range g for kv head
@@ -17,9 +18,9 @@
 // leaves partial rows that tree_combine_kernel joins.
 //
 // CTA:
-//   warps 0-7    two softmax streams, a thread a row (row = TMEM lane).  A stream's first thread
-//                also issues its tcgen05.mma: the stream has nothing else to do until its next
-//                scores are there, so no warp is spent on it.
+//   warps 0-7    two softmax streams, a thread a row (row = TMEM lane).  A thread of a stream's
+//                last warp also issues its tcgen05.mma: the stream has nothing else to do until its
+//                next scores are there, so no warp is spent on it.
 //   warps 8-     loaders, groups of four warps that take key tiles in turn: they load cache rows
 //                and convert them, K to [key][d], V to [d][key] (page-transposed Q8_0) or [key][d]
 //                (token rows).  A warp owns 32 keys of its tiles, so loading and converting need no

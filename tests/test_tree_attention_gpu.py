@@ -357,3 +357,27 @@ def test_pages_past_four_gigabytes(v_fmt):
     case.k_cache, case.v_cache = k, v
     case.bt = torch.where(case.bt >= 0, case.bt + first, case.bt)
     assert_close(case.run().float().cpu().numpy(), ref, what="far pages")
+
+
+@pytest.mark.parametrize("v_fmt", ["q8_0", "fp16"])
+def test_backend_forward_with_a_tree(v_fmt):
+    """Gfx906FAImpl.forward takes the bit rows from its metadata; the legacy mode, which has no Q8_0 cache, refuses them."""
+    pytest.importorskip("vllm")
+    import gfx906_fa_backend as be
+    case = TreeCase([500, 77], [12, 7], 48, 8, "q8t" if v_fmt == "q8_0" else "bf16", seed=28)
+    kv = torch.zeros((case.NB, 2, 16, 8, 128), dtype=torch.bfloat16, device=dev)
+    k, v = gfx906_fa_paged.kv_cache_views(kv, v_fmt)
+    k.copy_(case.k_cache)
+    v.copy_(case.v_cache)
+    impl = be.Gfx906FAImpl(num_heads=48, head_size=128, scale=case.scale, num_kv_heads=8, alibi_slopes=None, sliding_window=None,
+                           kv_cache_dtype="auto")
+    impl._v_fmt, impl._legacy = v_fmt, False
+    meta = be.Gfx906FAMetadata(num_actual_tokens=19, max_query_len=12, max_seq_len=500, query_start_loc=case.start,
+                               seq_lens=case.lens, block_table=case.bt, slot_mapping=torch.zeros(19, dtype=torch.int64, device=dev),
+                               tree_mask=case.mask)
+    out = torch.zeros((19, 48 * 128), dtype=torch.bfloat16, device=dev)
+    impl.forward(None, case.q, None, None, kv, meta, output=out)
+    assert_close(out.view(19, 48, 128).float().cpu().numpy(), case.reference(), what="backend")
+    impl._legacy = True
+    with pytest.raises(NotImplementedError):
+        impl.forward(None, case.q, None, None, kv, meta, output=out)
