@@ -683,6 +683,7 @@ struct ReadArgs {
   const int64_t* slots;
   int bs_log2, N, Hkv, out_dt, v_src;                       // v_src: DT_F16 / DT_BF16 of 16-bit V rows
   int k_w8, v_w8, v_w16, v_rec16;                  // rows on 8- and 16-byte boundaries, records on 16
+  uint32_t rows;                                   // rows the row items cover: N * Hkv keys, then as many values unless they go by runs
   uint32_t nrows, nruns;                           // row items (2 * RR rows a warp); run items follow
   void* k_out; void* v_out;                        // [N, Hkv, 128]; v_out may be null
 };
@@ -734,7 +735,7 @@ __global__ void __launch_bounds__(ns::WARPS * 32) read_kv_kernel(const __grid_co
       for (int k = 0; k < RR; ++k) {
         const uint32_t y = (it * RR + k) * 2 + (lane >> 4);
         isv[k] = y >= krows;
-        r[k] = isv[k] ? y - krows : y;
+        r[k] = y >= a.rows ? krows : isv[k] ? y - krows : y;           // past the last row: no row
         slot[k] = r[k] < krows ? a.slots[r[k] / (uint32_t)a.Hkv] : -1;
       }
       Q8Lane q[RR];
@@ -982,7 +983,8 @@ extern "C" cudaError_t gfx906_fa_read_kv(const G9KvCache* cache, int value_dtype
   const int64_t rows = (int64_t)num_rows * a.Hkv;
   if (rows >= 0x3fffffff) return cudaErrorInvalidValue;                // 32-bit row numbers
   const bool runs = value_out && cache->v_mode == G9_V_Q8T && a.v_rec16;
-  a.nrows = (uint32_t)((rows * (value_out && !runs ? 2 : 1) + 2 * RR - 1) / (2 * RR));
+  a.rows = (uint32_t)(rows * (value_out && !runs ? 2 : 1));
+  a.nrows = (a.rows + 2 * RR - 1) / (2 * RR);
   a.nruns = runs ? (uint32_t)((num_rows + 15) / 16) * a.Hkv : 0;
   const int64_t want = (int64_t)(a.nrows + a.nruns + ns::WARPS - 1) / ns::WARPS, cap = (int64_t)ns_sms() * 32;
   read_kv_kernel<<<(int)(want < cap ? want : cap), ns::WARPS * 32, 0, stream>>>(a);
