@@ -221,10 +221,10 @@ extern "C" cudaError_t gfx906_fa_move_kv(void* const* k_layers, void* const* v_l
   a.c = c; a.src = src_slots; a.dst = dst_slots; a.per = group_size;
   a.v_bytes = c.v_mode == G9_V_NONE ? 0 : c.v_mode == G9_V_COPY16 ? 2 * D : RB;
   a.k_w = width_of(km); a.v_w = width_of(vm);
-  // as many kv heads a CTA as shared memory holds; a group's rows of one head must fit
-  const int head_bytes = group_size * (RB + a.v_bytes);
-  a.heads = (kMoveSmem - 16 * group_size - 16) / (head_bytes > 0 ? head_bytes : 1);
-  if (a.heads < 1) return cudaErrorInvalidValue;
+  // as many kv heads a CTA as shared memory holds; a group's rows of one head must fit (in 64 bits: any group_size may be asked for)
+  const int64_t head_bytes = (int64_t)group_size * (RB + a.v_bytes), left = kMoveSmem - 16 * (int64_t)group_size - 16;
+  if (left < head_bytes) return cudaErrorInvalidValue;
+  a.heads = (int)(left / head_bytes);
   if (a.heads > c.num_heads_kv) a.heads = c.num_heads_kv;
   // few groups: halve the heads of a CTA until every SM has four
   int dev = 0, sms = 148;
