@@ -686,6 +686,7 @@ void check_index(const torch::Tensor& x, const char* name, c10::ScalarType dt, i
   TORCH_CHECK(x.device().is_cuda() && x.scalar_type() == dt && x.dim() == 1 && x.is_contiguous(), name,
               " must be a contiguous 1-D ", dt, " CUDA tensor");
   TORCH_CHECK(n < 0 || x.size(0) == n, name, " must have ", n, " entries, got ", x.size(0));
+  TORCH_CHECK(x.size(0) <= INT32_MAX, name, " must have at most ", INT32_MAX, " entries, got ", x.size(0));   // the C entries count in int
 }
 
 std::vector<torch::Tensor> tree_mask(torch::Tensor parents, torch::Tensor query_start_loc, torch::Tensor seq_lens,
