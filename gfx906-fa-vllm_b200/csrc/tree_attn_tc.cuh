@@ -779,6 +779,7 @@ __global__ void __launch_bounds__(tt::threads(NQ), 1) tree_tc_kernel(const __gri
               const float y = __uint_as_float(x[e]);
               x[e] = __float_as_uint(p.softcap > 0.f ? softcap_log2(y, a.cap_in, a.cap_out) : y * a.scale_log2);
             }
+            __syncwarp();                    // tanhf branches by lane; tensor-memory accesses are the whole warp's
             tmem_st8(tS + c * 8, x);
           }
           tmem_wait_st();
@@ -796,6 +797,7 @@ __global__ void __launch_bounds__(tt::threads(NQ), 1) tree_tc_kernel(const __gri
 #pragma unroll
             for (int e = 0; e < 32; ++e)
               if (!(v >> e & 1u)) x[e] = 0xff800000u;
+            __syncwarp();                    // the bit rows were read by lane
             tmem_st32(tS + c * 32, x);
           }
           tmem_wait_st();
@@ -930,6 +932,7 @@ __global__ void __launch_bounds__(tt::threads(NQ), 1) tree_tc_kernel(const __gri
         const int64_t ob = row_live ? o_offset(p, s.b, t, hq) : 0;
 #pragma unroll 1
         for (int c = c0; c < c1; ++c) {
+          __syncwarp();                      // rows past the group skip the stores below
           uint32_t o[32];
           tmem_ld32(tO + c * 32, o);
           tmem_wait_ld();
