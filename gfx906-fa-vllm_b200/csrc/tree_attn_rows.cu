@@ -4,7 +4,7 @@
 // or 16-byte (16-bit V, page-transposed V) boundaries that their copies need.
 //
 //   o_t = sum_k p_tk v_k,  p = softmax over the keys token t sees:
-//   context keys k < ctx (inside its window) and the drafts its bit row selects
+//   context keys k < ctx and the drafts its bit row selects, inside its window
 //
 // A warp per (token, query head): lane k of a 32-key step scores key k, the
 // running maximum and sum are kept in fp32, and lane l accumulates output
@@ -63,8 +63,9 @@ __global__ void __launch_bounds__(kRowWarps * 32) tree_rows_kernel(const __grid_
     const int k = k0 + lane;
     bool see = k < L;
     if (see) {
-      if (k < ctx) see = k >= lo;
+      if (k < ctx) see = true;
       else see = (tree_word(row, (k - ctx) >> 5, a.words, nq) >> ((k - ctx) & 31)) & 1;
+      see = see && k >= lo;
     }
     int phys = -1;
     if (see) {

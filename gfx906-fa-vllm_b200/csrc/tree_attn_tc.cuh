@@ -158,12 +158,12 @@ __device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 
 
 __device__ __forceinline__ uint32_t tree_sees(const int32_t* row, int words, int nq, int ctx, int lo, int base) {
   uint32_t v = low_bits(ctx - base);
-  if (lo > base) v &= ~low_bits(lo - base);
   const int j = base - ctx;                  // draft index of the first key
   if (j > -32 && j < nq) {
     if (j < 0) v |= tree_word(row, 0, words, nq) << -j;
     else v |= __funnelshift_r(tree_word(row, j >> 5, words, nq), tree_word(row, (j >> 5) + 1, words, nq), j & 31);
   }
+  if (lo > base) v &= ~low_bits(lo - base);
   return v;
 }
 

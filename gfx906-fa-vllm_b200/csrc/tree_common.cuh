@@ -35,13 +35,24 @@ __device__ __forceinline__ uint32_t tree_word(const int32_t* row, int w, int wor
   return left >= 32 ? x : x & ((1u << left) - 1u);
 }
 
-// First context key inside a row's window (INT_MIN without one).
+// First key inside a row's window (INT_MIN without one): a key's distance is
+// counted along the row's own path, the drafts it selects behind its context.
+// A path shorter than the window leaves some context in it; of a longer one the
+// last `window` drafts stay, and the first of them is the row's first key.
 __device__ __forceinline__ int tree_window_lo(const TreeArgs& a, const int32_t* row, int nq, int ctx) {
   if (a.p.window <= 0) return -0x7fffffff - 1;
   int seen = 0;
   for (int w = 0; 32 * w < nq; ++w) seen += __popc(tree_word(row, w, a.words, nq));
-  const int64_t lo = (int64_t)ctx + seen - a.p.window;
-  return lo < -0x7fffffff ? -0x7fffffff : (int)lo;
+  int drop = seen - a.p.window;              // drafts past the window
+  if (drop <= 0) {
+    const int64_t lo = (int64_t)ctx + drop;
+    return lo < -0x7fffffff ? -0x7fffffff : (int)lo;
+  }
+  int w = 0;
+  uint32_t x = tree_word(row, 0, a.words, nq);
+  for (; drop >= __popc(x); x = tree_word(row, ++w, a.words, nq)) drop -= __popc(x);
+  for (; drop > 0; --drop) x &= x - 1;
+  return ctx + 32 * w + __ffs(x) - 1;
 }
 
 }  // namespace g9

@@ -403,9 +403,10 @@ cudaError_t gfx906_fa_copy_pages(void* const* layers, int num_layers, int64_t nu
  * draft j (key ctx + j) iff bit j of its row is 1: row q_start[b] + t of
  * tree_mask (mask_words int32 a row, mask_row_stride int32 apart), or row
  * b * seq_q + t without q_start.  Draft keys past mask_words * 32 are hidden.
- * window > 0: a context key k is visible iff
- * ctx + (visible drafts - 1) - k < window, the distance along the token's own
- * path; drafts are governed by their bits alone.  A row that sees nothing is
+ * window > 0: of those, a key is visible iff its distance along the token's own
+ * path is below window, as in gfx906_fa_attention: the distance of draft j is
+ * the number of selected drafts behind it (j' > j), that of a context key k is
+ * ctx - k + (selected drafts) - 1.  A row that sees nothing is
  * written as zeros; a key no row's bits select never reaches that row, whatever its
  * cache row holds.  softcap, sinks, num_blocks, flags
  * (G9_F_CU_SEQLENS) and fp8 output as in gfx906_fa_attention.  workspace: at
