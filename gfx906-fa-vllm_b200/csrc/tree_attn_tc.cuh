@@ -824,6 +824,9 @@ __global__ void __launch_bounds__(tt::threads(NQ), 1) tree_tc_kernel(const __gri
           float alpha = 1.f;
           bool rescale = false;
           if (mx != -INFINITY && (m == -INFINITY || mx > m + kRescale)) {
+            // A whole number: weights already written are scaled by a power of two, which rounds none of them a second
+            // time, at the price of weights up to 2 times smaller (fp16 keeps 2^-24 of the largest).
+            mx = ceilf(mx);
             if (m != -INFINITY) {
               alpha = fast_exp2(m - mx);
               l *= alpha;
@@ -851,11 +854,10 @@ __global__ void __launch_bounds__(tt::threads(NQ), 1) tree_tc_kernel(const __gri
                 tmem_wait_st();
                 tmem_ld8(tS + c * 8, o);
                 tmem_wait_ld();
-                const __half2 a2 = __float2half2_rn(alpha);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                  const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&o[e]), a2);
-                  o[e] = *reinterpret_cast<const uint32_t*>(&y);
+                  const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&o[e]));
+                  o[e] = pack_half2(y.x * alpha, y.y * alpha);
                 }
                 tmem_st8(tS + c * 8, o);
               }
