@@ -33,6 +33,10 @@
 // the end.  NQ = 2 (more than 128 rows): the streams take one row tile each and share
 // every converted key tile.
 // Tensor memory: S0 S1 O0 O1, 128 columns each; P_i over the first half of S_i.
+// bf16 V stays bf16, whose range fp16 does not have; its MMA wants P in bf16 too, which keeps 8 bits
+// of a weight where fp16 keeps 11 (rows of few keys show it), so P is the sum of two bf16 terms (16 bits), multiplied
+// one after the other; they take all of S_i.  Against fp16 values (and their pass over every V tile): 32 sequences of
+// 1K-32K tokens 681 -> 724 us, 8 of 4K-16K with up to 60 drafts 290 -> 288 us.
 // Every mbarrier wait is bounded.
 //
 // 32 sequences of 1K-32K tokens, 16 drafts, 48/8 heads, Q8_0 V (1.19 GB): 485 us
@@ -191,10 +195,13 @@ __device__ __forceinline__ void dequant4(uint32_t x, __half2 s01, __half2 s23, u
   hi = *reinterpret_cast<const uint32_t*>(&q);
 }
 
+// exponent bits of a 16-bit value: all ones where it is not finite
+constexpr uint32_t exponent16(bool bf16) { return bf16 ? 0x7f80u : 0x7c00u; }
+
 // Clears the halves of w whose bit in `dead` is set and those that are not
-// finite; returns 1 if a live one was not finite.
+// finite (E: the type's exponent bits); returns 1 if a live one was not finite.
+template <uint32_t E>
 __device__ __forceinline__ int clean2(uint32_t& w, bool dead0, bool dead1) {
-  constexpr uint32_t E = 0x7c00u;
   int hit = 0;
   if (dead0) w &= 0xffff0000u;
   else if ((w & E) == E) { w &= 0xffff0000u; hit = 1; }
@@ -219,12 +226,11 @@ static __device__ __noinline__ bool tree_poisoned(const TreeArgs& a, const TreeS
       if (page_bad(p, phys)) continue;
       const int off = k % p.block_size, bs = p.block_size;
       const uint8_t* base = p.v_cache + (int64_t)phys * p.v_page_stride + (int64_t)h * p.v_head_stride;
+      const uint32_t E = exponent16(p.v_fmt == G9_VFMT_BF16);
       for (int d = 0; d < tt::D; ++d) {
-        __half v;
-        if (p.v_fmt == G9_VFMT_F16) {
-          v = reinterpret_cast<const __half*>(base + (int64_t)off * p.v_tok_stride)[d];
-        } else if (p.v_fmt == G9_VFMT_BF16) {
-          v = __float2half_rn(__bfloat162float(reinterpret_cast<const __nv_bfloat16*>(base + (int64_t)off * p.v_tok_stride)[d]));
+        uint16_t v;
+        if (p.v_fmt == G9_VFMT_F16 || p.v_fmt == G9_VFMT_BF16) {
+          v = reinterpret_cast<const uint16_t*>(base + (int64_t)off * p.v_tok_stride)[d];
         } else {
           const uint8_t *sc, *q;
           if (p.v_fmt == G9_VFMT_Q8T) {
@@ -234,9 +240,9 @@ static __device__ __noinline__ bool tree_poisoned(const TreeArgs& a, const TreeS
             sc = base + (int64_t)off * p.v_tok_stride + d / QK * QBLOCK;
             q = sc + 2 + d % QK;
           }
-          v = __hmul(__short2half_rn((short)*reinterpret_cast<const int8_t*>(q)), *reinterpret_cast<const __half*>(sc));
+          v = __half_as_ushort(__hmul(__short2half_rn((short)*reinterpret_cast<const int8_t*>(q)), *reinterpret_cast<const __half*>(sc)));
         }
-        if ((__half_as_ushort(v) & 0x7c00) == 0x7c00) return true;
+        if ((v & E) == E) return true;
       }
     }
   }
@@ -308,7 +314,7 @@ template <int NQ, int VF>
 __global__ void __launch_bounds__(tt::threads(NQ), 1) tree_tc_kernel(const __grid_constant__ TreeTcParams pp) {
   using namespace tt;
   constexpr int NT = threads(NQ), GROUPS = loader_groups(NQ);
-  constexpr bool DIRECT = VF == G9_VFMT_F16 || VF == G9_VFMT_BF16;
+  constexpr bool BF = VF == G9_VFMT_BF16, DIRECT = VF == G9_VFMT_F16 || BF;
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t sbase = smem_u32(smem);
   const uint32_t sK = sbase, sV = sK + ST * TILE, sQ = sV + ST * TILE;
@@ -603,7 +609,7 @@ __global__ void __launch_bounds__(tt::threads(NQ), 1) tree_tc_kernel(const __gri
             const uint4 x4 = *x;
             uint32_t o[4] = {x4.x, x4.y, x4.z, x4.w};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) hit |= clean2(o[e], 2 * e >= nv, 2 * e + 1 >= nv);
+            for (int e = 0; e < 4; ++e) hit |= clean2<exponent16(false)>(o[e], 2 * e >= nv, 2 * e + 1 >= nv);
             *x = make_uint4(o[0], o[1], o[2], o[3]);
           }
         }
@@ -622,9 +628,7 @@ __global__ void __launch_bounds__(tt::threads(NQ), 1) tree_tc_kernel(const __gri
             load_k();
           }
         }
-        // bf16 V becomes fp16 in place: exact for 2^-14 <= |v| < 65520, and P keeps fp16's 11 bits (in bf16 it would
-        // keep 8, which rows of few keys show)
-        if (VF == G9_VFMT_BF16 || checked) {
+        if (checked) {
           const int key = 32 * w + lane;
           const bool dead = lane >= valid;
 #pragma unroll 2
@@ -633,11 +637,7 @@ __global__ void __launch_bounds__(tt::threads(NQ), 1) tree_tc_kernel(const __gri
             const uint4 x4 = *x;
             uint32_t o[4] = {x4.x, x4.y, x4.z, x4.w};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              if constexpr (VF == G9_VFMT_BF16)
-                o[e] = pack_half2(__uint_as_float(o[e] << 16), __uint_as_float(o[e] & 0xffff0000u));
-              if (checked) hit |= clean2(o[e], dead, dead);
-            }
+            for (int e = 0; e < 4; ++e) hit |= clean2<exponent16(BF)>(o[e], dead, dead);
             *x = make_uint4(o[0], o[1], o[2], o[3]);
           }
         }
@@ -659,7 +659,8 @@ __global__ void __launch_bounds__(tt::threads(NQ), 1) tree_tc_kernel(const __gri
     const bool general = p.softcap > 0.f || !(p.scale > 0.f);
     const bool leader = (tid & 127) == 96;   // issues the stream's MMAs; its warp has no rows of its own below 97 of them
     constexpr uint32_t kS = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
-    constexpr uint32_t kPV = kS | (VF == G9_VFMT_Q8T ? 0u : 1u << 16);        // V by token rows: N-major
+    // V by token rows: N-major; bf16 V: both operands bf16
+    constexpr uint32_t kPV = kS | (VF == G9_VFMT_Q8T ? 0u : 1u << 16) | (BF ? 1u << 7 | 1u << 10 : 0u);
     const uint32_t qs = sQ + (NQ == 2 ? wi * TILE : 0);
     // Descriptors are advanced from one base each: the start address counts 16-byte units in the low bits.
     auto issue_s = [&](int n) {              // S = Q K(n)^T
@@ -678,7 +679,9 @@ __global__ void __launch_bounds__(tt::threads(NQ), 1) tree_tc_kernel(const __gri
 #pragma unroll
       for (int kk = 0; kk < BN / 16; ++kk) {
         const uint32_t off = (VF == G9_VFMT_Q8T ? (kk >> 2) * (TILE / 2) + (kk & 3) * 32 : kk * 2048) >> 4;
-        tc_mma_ts(tmem + 256 + wi * 128, tmem + wi * 128 + kk * 8, vd + off, kPV, (!first || kk > 0) ? 1u : 0u);
+        const uint32_t pa = tmem + wi * 128 + (BF ? (kk >> 2) * 64 + (kk & 3) * 8 : kk * 8);
+        tc_mma_ts(tmem + 256 + wi * 128, pa, vd + off, kPV, (!first || kk > 0) ? 1u : 0u);
+        if (BF) tc_mma_ts(tmem + 256 + wi * 128, pa + 32, vd + off, kPV, 1u);
       }
       tc_commit(&bpv[wi]);
       tc_commit(&vempty[n & 1]);
@@ -849,15 +852,19 @@ __global__ void __launch_bounds__(tt::threads(NQ), 1) tree_tc_kernel(const __gri
             }
             if (hf) {
 #pragma unroll 1
-              for (int c = 0; c < 4; ++c) {
+              for (int c = 0; c < (BF ? 8 : 4); ++c) {
                 uint32_t o[8];
                 tmem_wait_st();
                 tmem_ld8(tS + c * 8, o);
                 tmem_wait_ld();
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                  const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&o[e]));
-                  o[e] = pack_half2(y.x * alpha, y.y * alpha);
+                  if constexpr (BF) {        // either term
+                    o[e] = pack_bf162(__uint_as_float(o[e] << 16) * alpha, __uint_as_float(o[e] & 0xffff0000u) * alpha);
+                  } else {
+                    const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&o[e]));
+                    o[e] = pack_half2(y.x * alpha, y.y * alpha);
+                  }
                 }
                 tmem_st8(tS + c * 8, o);
               }
@@ -869,7 +876,7 @@ __global__ void __launch_bounds__(tt::threads(NQ), 1) tree_tc_kernel(const __gri
           uint64_t ls2[2] = {0ull, 0ull};
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            uint32_t pk[8];
+            uint32_t pk[8], lo[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
               const uint64_t y2 = f2fma(f2pack(__uint_as_float(x[c >> 1][(c & 1) * 16 + 2 * e]),
@@ -879,10 +886,16 @@ __global__ void __launch_bounds__(tt::threads(NQ), 1) tree_tc_kernel(const __gri
               y0 = fast_exp2(y0);
               y1 = fast_exp2(y1);
               ls2[e & 1] = f2add(ls2[e & 1], f2pack(y0, y1));
-              pk[e] = pack_half2(y0, y1);
+              if constexpr (BF) {
+                pk[e] = pack_bf162(y0, y1);
+                lo[e] = pack_bf162(y0 - __uint_as_float(pk[e] << 16), y1 - __uint_as_float(pk[e] & 0xffff0000u));
+              } else {
+                pk[e] = pack_half2(y0, y1);
+              }
             }
-            // 64 weights take 32 columns: columns whose scores this row has read
-            tmem_st8(tS + hf * 32 + c * 8, pk);
+            // 64 weights take 32 columns, two bf16 terms 64: columns whose scores this row has read
+            tmem_st8(tS + hf * (BF ? 64 : 32) + c * 8, pk);
+            if constexpr (BF) tmem_st8(tS + hf * 64 + 32 + c * 8, lo);
           }
           float a0, a1, b0, b1;
           f2unpack(ls2[0], a0, a1);
