@@ -146,6 +146,7 @@ static bool tree_batch_ok(const G9AttnBatch& p) {
   if (p.q_dtype < 0 || p.q_dtype > 2 || p.out_dtype < 0 || p.out_dtype > 3 || p.v_fmt < 0 || p.v_fmt > 3) return false;
   if (p.out_dtype == G9_DT_FP8E4M3 && !p.out_scale) return false;
   if (p.q_abs || p.mask || (p.flags & G9_F_CAUSAL_END)) return false;
+  if ((p.flags & G9_F_CU_SEQLENS) && !p.n_q && !p.q_start) return false;     // drafts are counted from q_start
   if (((uintptr_t)p.k_cache | (uintptr_t)p.k_page_stride | (uintptr_t)p.k_tok_stride | (uintptr_t)p.k_head_stride) & 1) return false;
   uintptr_t v = (uintptr_t)p.v_cache | (uintptr_t)p.v_page_stride | (uintptr_t)p.v_head_stride;
   if (p.v_fmt != G9_VFMT_Q8T) v |= (uintptr_t)p.v_tok_stride;
