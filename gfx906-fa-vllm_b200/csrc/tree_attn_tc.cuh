@@ -98,7 +98,7 @@ __device__ __forceinline__ TreeShape tree_shape(const TreeArgs& a, int b) {
   s.R = s.nq * a.G;
   s.groups = (s.R + NQ * tt::BM - 1) / (NQ * tt::BM);
   // first context key any row's window can hold (a row sees at least no draft: depth -1)
-  const int lo = a.p.window > 0 ? max(0, s.ctx - a.p.window) : 0;
+  const int lo = a.p.window > 0 && s.ctx > a.p.window ? s.ctx - a.p.window : 0;
   s.j0 = lo / tt::BN;
   s.tiles = max(1, (s.L + tt::BN - 1) / tt::BN - s.j0);
   return s;

@@ -62,3 +62,14 @@ def test_any_bits_keep_the_last_ones(window):
     seen = [f & (np.cumsum(f[:, ::-1], 1)[:, ::-1] <= window) for f in full]
     case = TreeCase([370, 9, 60], [70, 9, 4], 12, 2, "q8t", seed=window, seen=full)
     check(case, seen, window, f"any bits, window {window}")
+
+
+@pytest.mark.parametrize("bs", [16, 8])
+def test_a_window_wider_than_any_length_hides_nothing(bs):
+    """Sequences of which the cache holds fewer rows than they drafted stand before position 0; with the widest window too."""
+    case = TreeCase([12, 40, 300], [12, 40, 9], 12, 2, "q8t", bs=bs, seed=3)
+    case.lens = torch.tensor([3, 0, 300], dtype=torch.int32, device=dev)
+    ref = case.run()
+    assert torch.isfinite(ref).all() and ref[52:].any()
+    assert torch.equal(case.run(sliding_window=2 ** 31 - 1), ref)
+    assert torch.equal(case.run(sliding_window=2 ** 31 - 20), ref)
