@@ -18,6 +18,7 @@
 
 #include "common.cuh"
 #include "gfx906_fa_b200.h"
+#include "q8_quant.cuh"
 #include "tcgen05.cuh"
 
 namespace g9 {
@@ -172,32 +173,16 @@ __device__ __forceinline__ uint2 quant8(const float v[8], uint16_t& scale) {
   return make_uint2(w[0], w[1]);
 }
 
-// The same for elements that are fp16 or bf16 values, without the division
-// routine and the conversions: amax / 127 as a product with 1/127 and one
-// residual step, and the nearest integer by adding 1.5 * 2^23 (ties to even),
-// both exact for such values (the KV store's tests check every 16-bit maximum).
+// The same for elements that are fp16 or bf16 values.
 __device__ __forceinline__ uint2 quant8_16bit(const float v[8], uint16_t& scale) {
   float amax = fabsf(v[0]);
 #pragma unroll
   for (int e = 1; e < 8; ++e) amax = fmaxf(amax, fabsf(v[e]));
   amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
   amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-  constexpr float kInv127 = 1.0f / 127.0f;
-  const float y = __fmul_rn(amax, kInv127);
-  const float d = fmaf(fmaf(-y, 127.0f, amax), kInv127, y);
-  const float id = d > 0.0f ? __frcp_rn(d) : 0.0f;
-  constexpr float kMagic = 12582912.0f;
-  uint32_t b[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    float r = __fadd_rn(__fmul_rn(v[e], id), kMagic);
-    r = r == r ? r : kMagic;                         // 0 * inf: a scale that underflowed
-    r = fminf(fmaxf(r, kMagic - 128.0f), kMagic + 127.0f);
-    b[e] = __float_as_uint(r);
-  }
-  scale = __half_as_ushort(__float2half_rn(d));
-  return make_uint2(__byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410),
-                    __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410));
+  float id;
+  scale = __half_as_ushort(__float2half_rn(q8_scale_16bit(amax, id)));
+  return make_uint2(q8_quants4(v[0], v[1], v[2], v[3], id), q8_quants4(v[4], v[5], v[6], v[7], id));
 }
 
 // cos / sin of this lane's 8 elements.  NeoX: element e pairs with e +- rot/2;

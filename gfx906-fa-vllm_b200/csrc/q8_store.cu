@@ -23,6 +23,7 @@
 //     to Q8_0 with the same rules as K.
 #include "common.cuh"
 #include "gfx906_fa_b200.h"
+#include "q8_quant.cuh"
 
 namespace g9 {
 
@@ -250,36 +251,9 @@ __global__ void __launch_bounds__(kWarps * 32) q8_store_fast_kernel(StoreArgs a)
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 4));
-      // amax / 127 correctly rounded without the IEEE division routine:
-      // y = amax * fl(1/127), then one residual-correction step of the
-      // reciprocal product (Markstein's method: r = amax - y*127 exactly by
-      // FMA, y' = y + r*fl(1/127)).  Exact for every finite fp16 and bf16
-      // value, which are all the values amax can take here (16-bit inputs);
-      // tests/test_store_gpu.py::test_fast_store_every_16bit_absmax checks
-      // all of them on the GPU against the oracle's IEEE division.
-      constexpr float kInv127 = 1.0f / 127.0f;
-      const float y127 = __fmul_rn(amax, kInv127);
-      const float dq = fmaf(fmaf(-y127, 127.0f, amax), kInv127, y127);
-      const float id = dq > 0.0f ? __frcp_rn(dq) : 0.0f;
-      // rint(v*id) clamped to [-128, 127] without the (quarter-rate)
-      // float->int conversion: the product is rounded to fp32 as in the
-      // reference, then adding 1.5*2^23 rounds it to an integer with ties to
-      // even (exactly rintf for |x| < 2^22) and leaves it in the low mantissa
-      // bits; the clamp is applied to the sum, and the int8 is its low byte.
-      // Identical to the general kernel for finite inputs.  When the block's
-      // scale underflows so far that 1/d is infinite, a zero element gives
-      // 0 * inf = NaN: it becomes 0, as the general kernel's float -> int
-      // conversion (and the reference's) makes it; +-inf products clamp.
-      constexpr float kMagic = 12582912.0f;
-      uint32_t rb[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float r = __fadd_rn(__fmul_rn(v[e], id), kMagic);
-        r = r == r ? r : kMagic;
-        r = fminf(fmaxf(r, kMagic - 128.0f), kMagic + 127.0f);
-        rb[e] = __float_as_uint(r);
-      }
-      const uint32_t packed = __byte_perm(__byte_perm(rb[0], rb[1], 0x0040), __byte_perm(rb[2], rb[3], 0x0040), 0x5410);
+      float id;
+      const float dq = q8_scale_16bit(amax, id);
+      const uint32_t packed = q8_quants4(v[0], v[1], v[2], v[3], id);
       uint8_t* out = stage + i * kFastRowBytes + (lane >> 3) * QBLOCK;
       uint16_t* o16 = reinterpret_cast<uint16_t*>(out + 2 + 4 * (lane & 7));
       o16[0] = (uint16_t)(packed & 0xffffu);
@@ -348,21 +322,9 @@ __global__ void __launch_bounds__(kWarps * 32) q8_store_fast16_kernel(StoreArgs 
       for (int e = 1; e < 8; ++e) amax = fmaxf(amax, fabsf(v[e]));
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-      constexpr float kInv127 = 1.0f / 127.0f;
-      const float y127 = __fmul_rn(amax, kInv127);
-      const float dq = fmaf(fmaf(-y127, 127.0f, amax), kInv127, y127);
-      const float id = dq > 0.0f ? __frcp_rn(dq) : 0.0f;
-      constexpr float kMagic = 12582912.0f;
-      uint32_t rb[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        float r = __fadd_rn(__fmul_rn(v[e], id), kMagic);
-        r = r == r ? r : kMagic;
-        r = fminf(fmaxf(r, kMagic - 128.0f), kMagic + 127.0f);
-        rb[e] = __float_as_uint(r);
-      }
-      const uint32_t p0 = __byte_perm(__byte_perm(rb[0], rb[1], 0x0040), __byte_perm(rb[2], rb[3], 0x0040), 0x5410);
-      const uint32_t p1 = __byte_perm(__byte_perm(rb[4], rb[5], 0x0040), __byte_perm(rb[6], rb[7], 0x0040), 0x5410);
+      float id;
+      const float dq = q8_scale_16bit(amax, id);
+      const uint32_t p0 = q8_quants4(v[0], v[1], v[2], v[3], id), p1 = q8_quants4(v[4], v[5], v[6], v[7], id);
       const int r = 2 * k + half;
       uint8_t* out = stage + r * kFastRowBytes + (hl >> 2) * QBLOCK;
       uint16_t* o16 = reinterpret_cast<uint16_t*>(out + 2 + 8 * (hl & 3));
