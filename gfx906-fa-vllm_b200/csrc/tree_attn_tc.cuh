@@ -887,8 +887,15 @@ __global__ void __launch_bounds__(tt::threads(NQ), 1) tree_tc_kernel(const __gri
               y1 = fast_exp2(y1);
               ls2[e & 1] = f2add(ls2[e & 1], f2pack(y0, y1));
               if constexpr (BF) {
-                pk[e] = pack_bf162(y0, y1);
-                lo[e] = pack_bf162(y0 - __uint_as_float(pk[e] << 16), y1 - __uint_as_float(pk[e] & 0xffff0000u));
+                // Upper halves, and what is left of y * (1 + 2^-23): never 0 where y is not, so that an infinite value
+                // meets two weights of one sign and stays infinite
+                const uint32_t b0 = __float_as_uint(y0), b1 = __float_as_uint(y1);
+                pk[e] = __byte_perm(b0, b1, 0x7632);
+                constexpr uint32_t H = 0xffff0000u, S = 0x80000000u;
+                float l0, l1;
+                f2unpack(f2fma(f2pack(y0, y1), f2pack(1.f + 0x1p-23f, 1.f + 0x1p-23f),
+                               f2pack(__uint_as_float((b0 & H) | S), __uint_as_float((b1 & H) | S))), l0, l1);
+                lo[e] = pack_bf162(l0, l1);
               } else {
                 pk[e] = pack_half2(y0, y1);
               }

@@ -46,3 +46,20 @@ def test_bf16_values_do_not_depend_on_the_caches_alignment():
         case.run(out=other)
         assert_close((out / scale).cpu().numpy(), (other / scale).cpu().numpy(), what=f"{scale}")
         case.v_cache = value
+
+
+def test_an_infinite_bf16_value_stays_infinite():
+    """In a tile that every row sees whole, also where every weight is exactly 1 (equal scores: keys of zero)."""
+    for keys in (1.0, 0.0):
+        case = TreeCase([400], [9], 12, 2, "bf16", seed=4, dtype=torch.bfloat16)
+        if keys == 0:
+            case.k_cache.zero_()
+        page = case.block_table[0].tolist()
+        for pos, d, x in ((5, 3, float("inf")), (140, 40, -float("inf")), (141, 90, float("nan")), (6, 91, float("inf")),
+                          (142, 91, -float("inf"))):
+            case.v_cache[page[pos // 16], pos % 16, :, d] = x
+        out = case.run().float().cpu()
+        assert (out[..., 3] == float("inf")).all() and (out[..., 40] == -float("inf")).all()
+        assert out[..., 90:92].isnan().all()
+        rest = [d for d in range(128) if d not in (3, 40, 90, 91)]
+        assert_close(out[..., rest].numpy(), case.reference()[..., rest], what="the other elements")
