@@ -211,10 +211,12 @@ __device__ __forceinline__ int clean2(uint32_t& w, bool dead0, bool dead1) {
 }
 
 // Rare: a tile whose keys are checked held a value that is not finite.  The
-// converters cleared it, so that rows which do not see the key stay clean; a
-// row that sees such a key is not a number.
-static __device__ __noinline__ bool tree_poisoned(const TreeArgs& a, const TreeSeg& s, int h, const int32_t* row, int lo) {
+// converters cleared it, so that rows which do not see the key stay clean;
+// here is what a row that sees such keys has lost of elements d0 .. d0 + 31: bits
+// of those that met +infinity (x) and -infinity (y), both for not a number.
+static __device__ __noinline__ uint2 tree_lost(const TreeArgs& a, const TreeSeg& s, int h, const int32_t* row, int lo, int d0) {
   const G9AttnBatch& p = a.p;
+  uint2 lost = make_uint2(0u, 0u);
   for (int j = s.j; j < s.j + s.n; ++j) {
     bool checked = tree_checked(a, s, j * tt::BN);         // or a page of it is not there
     for (int k = j * tt::BN; !checked && k < min(s.L, (j + 1) * tt::BN); k += 16)
@@ -227,7 +229,8 @@ static __device__ __noinline__ bool tree_poisoned(const TreeArgs& a, const TreeS
       const int off = k % p.block_size, bs = p.block_size;
       const uint8_t* base = p.v_cache + (int64_t)phys * p.v_page_stride + (int64_t)h * p.v_head_stride;
       const uint32_t E = exponent16(p.v_fmt == G9_VFMT_BF16);
-      for (int d = 0; d < tt::D; ++d) {
+      for (int i = 0; i < 32; ++i) {
+        const int d = d0 + i;
         uint16_t v;
         if (p.v_fmt == G9_VFMT_F16 || p.v_fmt == G9_VFMT_BF16) {
           v = reinterpret_cast<const uint16_t*>(base + (int64_t)off * p.v_tok_stride)[d];
@@ -242,11 +245,14 @@ static __device__ __noinline__ bool tree_poisoned(const TreeArgs& a, const TreeS
           }
           v = __half_as_ushort(__hmul(__short2half_rn((short)*reinterpret_cast<const int8_t*>(q)), *reinterpret_cast<const __half*>(sc)));
         }
-        if ((v & E) == E) return true;
+        if ((v & E) != E) continue;
+        const bool nan = (v & ~E & 0x7fffu) != 0;
+        if (nan || !(v >> 15)) lost.x |= 1u << i;
+        if (nan || v >> 15) lost.y |= 1u << i;
       }
     }
   }
-  return false;
+  return lost;
 }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
@@ -322,7 +328,7 @@ __global__ void __launch_bounds__(tt::threads(NQ), 1) tree_tc_kernel(const __gri
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + smem_bar_off(NQ));
   uint64_t *kfull = bars, *kempty = bars + 2, *vfull = bars + 4, *vempty = bars + 6, *qfull = bars + 8, *bs_ = bars + 10,
            *bp = bars + 12, *bo = bars + 14, *bx = bars + 16, *by = bars + 17, *bpv = bars + 18, *vraw = bars + 20;
-  int* misc = reinterpret_cast<int*>(bars + 28);     // 0: tensor memory, 1: abort, 2: poison, 4: b, 5: base, 8..23: scan
+  int* misc = reinterpret_cast<int*>(bars + 28);     // 0: tensor memory, 1: abort, 2: a value was not finite, 4: b, 5: base, 8..23: scan
   uint32_t* tilebad = reinterpret_cast<uint32_t*>(misc + 24);                // [8], a byte per 32 keys
 
   const TreeArgs& a = pp.a;
@@ -938,7 +944,6 @@ __global__ void __launch_bounds__(tt::threads(NQ), 1) tree_tc_kernel(const __gri
         l = (use0 ? l * w0 : 0.f) + (use1 ? l1 * w1 : 0.f);
         m = top;
       }
-      if (row_live && misc[2] && tree_poisoned(a, s, h, bits, lo)) l = __int_as_float(0x7fffffff);
       if (warp_live && stream_on) {
         const bool whole = s.part < 0;
         const bool any = l > 0.f || l != l;
@@ -954,6 +959,8 @@ __global__ void __launch_bounds__(tt::threads(NQ), 1) tree_tc_kernel(const __gri
         const int64_t ob = row_live ? o_offset(p, s.b, t, hq) : 0;
 #pragma unroll 1
         for (int c = c0; c < c1; ++c) {
+          uint2 lost = make_uint2(0u, 0u);
+          if (row_live && misc[2]) lost = tree_lost(a, s, h, bits, lo, c * 32);
           __syncwarp();                      // rows past the group skip the stores below
           uint32_t o[32];
           tmem_ld32(tO + c * 32, o);
@@ -969,6 +976,15 @@ __global__ void __launch_bounds__(tt::threads(NQ), 1) tree_tc_kernel(const __gri
               if (use1) o[e] = __float_as_uint(__uint_as_float(o[e]) + __uint_as_float(q[e]) * w1);
           }
           if (!row_live) continue;
+          if (lost.x | lost.y) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              float x = __uint_as_float(o[e]);
+              if (lost.x >> e & 1u) x += INFINITY;
+              if (lost.y >> e & 1u) x -= INFINITY;
+              o[e] = __float_as_uint(x);
+            }
+          }
           if (!whole) {
             float* dst = pp.po + (slot * D + c * 32) * pp.rc + rl;
 #pragma unroll
