@@ -12,10 +12,11 @@
 //
 // copy_pages: whole pages, for a fork's last partly filled page or a swap.
 //
-// Both move bytes.  500 pages of 64 KB in 16 layers: 155 us, 6.8 TB/s, HBM.  8
-// rows of 128 sequences in 32 layers (206 MB of 136- and 256-byte rows): 51 us,
-// bound by the two round trips of a CTA.  Few rows: one launch and the same two
-// round trips, 10 us.  Layer addresses travel as kernel parameters, so a call
+// Both move bytes; L2 flushed before: 500 pages of 64 KB in 16 layers 166 us,
+// 6.3 TB/s, HBM.  8 rows of 128 sequences in 32 layers (206 MB of 136- and 256-byte
+// rows) 55 us, bound by the two round trips of a CTA; with page-transposed V
+// (143 MB) 301 us, bound by its byte accesses, 16 apart.  Few rows: one launch and
+// the same two round trips, 10 us.  Layer addresses travel as kernel parameters, so a call
 // needs no device-side table.
 #include <type_traits>
 

@@ -11,7 +11,8 @@
 // load per lane, the mean of squares four shuffles and a Q8_0 block's maximum
 // two.  All arithmetic is fp32.  Queries and keys are read and written once,
 // where separate norm, rotation and store passes move them three times.
-// 16384 tokens of 48 + 8 heads (505 MB): 140 us, 3.6 TB/s.  Bound by what 24
+// 16384 tokens of 48 + 8 heads (505 MB, L2 flushed before): 147 us, 3.4 TB/s; with
+// token-row Q8_0 V 145 us, 16-bit V (521 MB) 141 us, 3.7 TB/s.  Bound by what 24
 // warps an SM keep in flight between their dependent loads (position, angles,
 // rows), with half the issue slots taken: 127 instructions a pair of query rows.
 #include <cstdlib>
@@ -368,9 +369,9 @@ __global__ void __launch_bounds__(ns::WARPS * 32) norm_store_kernel(const __grid
 
 // ---------------------------------------------------------------------------
 // 16-bit tensors of one type on 16-byte rows, 8-byte cache rows: what a model
-// serves.  Three CTAs an SM at 80 registers: two took 228 us where three took
-// 193 for 16384 tokens and their read back; four spill (175 against 179 now, but
-// 37 against 29 at 2111 tokens).  Queries, keys and values are separate warp items, so that no warp
+// serves.  Three CTAs an SM at 80 registers: with two, 16384 tokens and their read
+// back took 1.18 times as long; four spill (0.98 times there, but 1.28 times at
+// 2111 tokens).  Queries, keys and values are separate warp items, so that no warp
 // carries another operand's code: a query item is QR rows of a token (their
 // angles loaded once), a key item its kv heads, a value item a run of slots
 // (page-transposed) or a token's heads.
@@ -701,7 +702,8 @@ __device__ __forceinline__ void q8_values(const Q8Lane& x, int hl, bool w8, floa
   for (int e = 0; e < 8; ++e) v[e] = (float)(int8_t)(q >> (8 * e)) * d;
 }
 
-// 16384 rows of 8 heads: 37 us for 103 MB.  Row items: half a warp reads RR rows.  Run items: page-transposed V by
+// 16384 rows of 8 heads (L2 flushed before): 43 us for 103 MB with page-transposed V, 58 us for 118 MB with 16-bit V, 59 us
+// for 103 MB with token-row Q8_0 V: latency, nothing of an item is asked for before the one before it is done.  Row items: half a warp reads RR rows.  Run items: page-transposed V by
 // runs of slots (run_bits): a lane takes 4 dims x 16 tokens as four 16-byte
 // loads, whatever part of the 16 the run covers.
 __global__ void __launch_bounds__(ns::WARPS * 32) read_kv_kernel(const __grid_constant__ ReadArgs a) {
@@ -918,7 +920,7 @@ extern "C" cudaError_t gfx906_fa_norm_rope_store_kv(
   if (fast) {
     FastItems f{};
     // Few tokens: 8 query rows a warp, so that more SMs have work.  Many: a token's queries, which share its angles and the
-    // weights (16384 tokens of 48 + 8 heads, the whole call with its read back: 16 rows an item 204 us, a token's queries 193 us).
+    // weights (16384 tokens of 48 + 8 heads, the call and its read back: 16 rows an item take 1.06 times as long).
     f.qr = (int64_t)num_tokens * a.Hq < (int64_t)sms * ns::WARPS * 32 ? 8 : (a.Hq + 7) / 8 * 8;
     f.pq = (a.Hq + f.qr - 1) / f.qr;
     f.pk = (a.Hkv + 7) / 8;

@@ -8,7 +8,9 @@
 //
 // A warp per (token, query head): lane k of a 32-key step scores key k, the
 // running maximum and sum are kept in fp32, and lane l accumulates output
-// elements 4l .. 4l+3.
+// elements 4l .. 4l+3.  Every head and draft reads its keys anew: 4 sequences of
+// 1K-4K tokens, 16 drafts, 48/8 heads take 3.9 ms, where the tensor-core kernel
+// takes 46 us on a cache that it can read.
 #include <algorithm>
 
 #include "tree_attn_tc.cuh"

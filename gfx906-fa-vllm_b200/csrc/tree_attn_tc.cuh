@@ -39,11 +39,13 @@
 // 1K-32K tokens 681 -> 724 us, 8 of 4K-16K with up to 60 drafts 290 -> 288 us.
 // Every mbarrier wait is bounded.
 //
-// 32 sequences of 1K-32K tokens, 16 drafts, 48/8 heads, Q8_0 V (1.19 GB): 485 us
-// at full clocks, 2.4 TB/s, 314 TFLOP/s; 530 us sustained.  A stream's chain of softmax, PV and
+// 32 sequences of 1K-32K tokens, 16 drafts, 48/8 heads, Q8_0 V (1.19 GB): 496 us
+// for a call by itself, 2.4 TB/s, 307 TFLOP/s; 500-535 us in a row of them.  Token-row Q8_0 V 532 us, fp16
+// V (1.7 GB) 628 us; 64/8 heads 499 us, 128/8 heads 853 us; a soft-cap 941 us (another pass over the scores, and its tanh);
+// a window of 1024 keys 83 us.  A stream's chain of softmax, PV and
 // next scores takes 6300 cycles for two tiles, the loaders 6200, so neither the
 // tensor core (1000 busy cycles a tile) nor HBM (1500) is the bound.  8 sequences
-// of 4K-16K, up to 60 drafts, fp16 V: 232 us, 398 TFLOP/s, the softmax of two row tiles.
+// of 4K-16K, up to 60 drafts, fp16 V: 235-245 us, 390 TFLOP/s, the softmax of two row tiles.
 #pragma once
 
 #include "tcgen05.cuh"
@@ -184,7 +186,9 @@ __device__ __forceinline__ uint64_t sw128_desc_mn(uint32_t saddr, uint32_t half)
   return d;
 }
 
-// int8 x 4 (packed) -> two fp16x2 times scale, one rounding.
+// int8 x 4 (packed) -> two fp16x2 times scale, one rounding: scales differ by 32-element block, so they cannot be applied to a
+// score that is one product over 128 elements, and a second term for what rounding leaves would double a K tile's shared
+// memory, of which 16 to 27 KB are left.  2^-12 of each element; with fp16 output the whole error is 4e-4 where fp32 operands leave 2e-4.
 __device__ __forceinline__ void dequant4(uint32_t x, __half2 s01, __half2 s23, uint32_t& lo, uint32_t& hi) {
   x ^= 0x80808080u;
   const uint32_t a = __byte_perm(x, 0x64646464u, 0x5140), b = __byte_perm(x, 0x64646464u, 0x5342);

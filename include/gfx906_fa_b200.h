@@ -334,7 +334,8 @@ typedef struct G9KvCache {
   uint8_t* v;
   int64_t v_page_stride, v_tok_stride, v_head_stride;
   int v_mode;
-  int num_blocks; /* slots at or past num_blocks * block_size are skipped and set bit 3 of the error word */
+  int num_blocks; /* slots at or past num_blocks * block_size are skipped and set bit 3 of the error word (0: not
+                     checked; gfx906_fa_move_kv wants it) */
   int block_size;
   int num_heads_kv;
 } G9KvCache;
